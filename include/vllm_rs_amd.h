@@ -169,6 +169,30 @@ void vra_dense_frag_gemm(const void* x, const void* wd, const void* bias, const 
 void vra_dense_frag_gemm_segments(const void* x, const void* wd, const void* const* bias, const int32_t* n, int32_t nseg, void* const* out, int32_t m,
                                   int32_t k, int32_t dtype, int32_t tile_n, int64_t stream);
 
+/* W8A8: linear layers in 8-bit integers, a scale a token for the activations and a scale a channel for the weights (the reference has 4-bit weights with
+ * 16-bit activations only; no call of its own stands behind these).
+ * Rows to 8 bits: q[t, c] = rint(127 p / a), a = max_c |p|, scales[t] = a / 127, with p = x (vra_quant_rows_i8), p = x weight (vra_rms_norm_i8) or
+ * p = h weight, h = round(x + residual), written to h_out (vra_add_rms_norm_i8; h_out may be x or residual); behind a norm scales[t] is a / (127 sqrt(mean_c h^2 + eps)).
+ * q is the correctly rounded quotient (ties to even) of the products p, which are formed in f32 (exact where they are normal numbers of it).  A row of zeros:
+ * scale 0; a row in which x, the sum or a product is not finite in f32: codes 0, scale NaN, and so NaN in every product of it.  The mean is formed in f64.
+ * x, residual, weight, h_out: bf16/f16, contiguous, 1..131072 columns, on any element. */
+void vra_quant_rows_i8(const void* x, int8_t* q, float* scales, int32_t rows, int32_t cols, int32_t dtype, int64_t stream);
+void vra_rms_norm_i8(const void* x, const void* weight, int8_t* q, float* scales, int32_t tokens, int32_t hidden, float eps, int32_t dtype,
+                     int64_t stream);
+void vra_add_rms_norm_i8(const void* x, const void* residual, const void* weight, void* h_out, int8_t* q, float* scales, int32_t tokens,
+                         int32_t hidden, float eps, int32_t dtype, int64_t stream);
+/* out[m, n] = round(x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n] + residual[m, n]): w row-major [n, k] as stored in the checkpoint, x and w any
+ * 8-bit integers (-128 too), any k up to 131071, sums in 32-bit integers (exact), everything behind them in f32 with one rounding.  dtype (bf16/f16/f32): of bias [n]
+ * and residual [m, n] (both nullable) and out; residual may be out.  Nothing but out's m rows is written, besides the workspace. */
+void vra_w8a8_gemm(const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales, const void* bias, const void* residual, void* out,
+                   void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream);
+/* the gate / up pair of a feed-forward block (mlp.rs:451-469): out[m, n] = round(silu(g) u), g and u two such products in f32; dtype bf16/f16 */
+void vra_w8a8_gate_up_silu(const int8_t* x, const float* x_scales, const int8_t* w_gate, const float* s_gate, const int8_t* w_up, const float* s_up,
+                           void* out, void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream);
+/* `workspace` of both: this many bytes on a multiple of 16, zeroed ONCE by the caller, one per concurrent stream (a captured graph counts as the stream it is replayed
+ * on); products of few rows split K over workgroups that meet in it.  Null: no such split; the results are the same bits either way. */
+size_t vra_w8a8_workspace_bytes(void);
+
 /* candle_nn::RmsNorm::forward as used by NormX (src/models/layers/others.rs:11-29):
  * out[t,:] = x[t,:] * rsqrt(mean(x²)+eps) * w, f32 math, one rounding. */
 void vra_rms_norm(const void* x, const void* weight, void* out, int32_t tokens, int32_t hidden,

@@ -237,6 +237,50 @@ def argmax(logits, rows, cols):
     return out.numpy(np.uint32, (rows,))
 
 
+# ---------------------------------------------------------------- W8A8: 8-bit integers, a scale a token and a scale a channel
+def quant_rows_i8(x, rows, cols, dtype=BF16):
+    """rows in 8 bits -> (q [rows, cols] int8, scales [rows] f32)"""
+    q, scales = DevBuf(rows * cols), DevBuf(rows * 4)
+    lib().vra_quant_rows_i8(_ptr(x), q.ptr, scales.ptr, rows, cols, dtype, 0)
+    check_error()
+    return q, scales
+
+
+def rms_norm_i8(x, weight, tokens, hidden, eps, dtype=BF16):
+    """rms_norm with its output in 8 bits -> (q, scales)"""
+    q, scales = DevBuf(tokens * hidden), DevBuf(tokens * 4)
+    lib().vra_rms_norm_i8(_ptr(x), _ptr(weight), q.ptr, scales.ptr, tokens, hidden, eps, dtype, 0)
+    check_error()
+    return q, scales
+
+
+def add_rms_norm_i8(x, residual, weight, tokens, hidden, eps, dtype=BF16):
+    """add_rms_norm with its output in 8 bits -> (h, q, scales)"""
+    h, q, scales = DevBuf(tokens * hidden * 2), DevBuf(tokens * hidden), DevBuf(tokens * 4)
+    lib().vra_add_rms_norm_i8(_ptr(x), _ptr(residual), _ptr(weight), h.ptr, q.ptr, scales.ptr, tokens, hidden, eps, dtype, 0)
+    check_error()
+    return h, q, scales
+
+
+class W8A8:
+    """products of 8-bit rows (vra_w8a8_gemm, vra_w8a8_gate_up_silu); owns the zeroed workspace that the launches of one stream share"""
+
+    def __init__(self):
+        self.ws = DevBuf(lib().vra_w8a8_workspace_bytes()).zero()
+
+    def gemm(self, x, x_scales, w, w_scales, m, k, n, bias=None, residual=None, dtype=BF16):
+        out = DevBuf(m * n * (4 if dtype == F32 else 2))
+        lib().vra_w8a8_gemm(_ptr(x), _ptr(x_scales), _ptr(w), _ptr(w_scales), _ptr(bias), _ptr(residual), out.ptr, self.ws.ptr, m, k, n, dtype, 0)
+        check_error()
+        return out
+
+    def gate_up_silu(self, x, x_scales, w_gate, s_gate, w_up, s_up, m, k, n, dtype=BF16):
+        out = DevBuf(m * n * 2)
+        lib().vra_w8a8_gate_up_silu(_ptr(x), _ptr(x_scales), _ptr(w_gate), _ptr(s_gate), _ptr(w_up), _ptr(s_up), out.ptr, self.ws.ptr, m, k, n, dtype, 0)
+        check_error()
+        return out
+
+
 # ---------------------------------------------------------------- rotary_emb.rs / attention.rs mirror
 class FusedRope:
     """attention_rs::fused_rope::FusedRope (rotary_emb.rs:88-103)."""
