@@ -182,13 +182,20 @@ void vra_rms_norm_i8(const void* x, const void* weight, int8_t* q, float* scales
 void vra_add_rms_norm_i8(const void* x, const void* residual, const void* weight, void* h_out, int8_t* q, float* scales, int32_t tokens,
                          int32_t hidden, float eps, int32_t dtype, int64_t stream);
 /* out[m, n] = round(x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n] + residual[m, n]): w row-major [n, k] as stored in the checkpoint, x and w any
- * 8-bit integers (-128 too), any k up to 131071, sums in 32-bit integers (exact), everything behind them in f32 with one rounding.  dtype (bf16/f16/f32): of bias [n]
+ * 8-bit integers (-128 too), any k up to 131071 and n up to 2^24, sums in 32-bit integers (exact), everything behind them in f32 with one rounding.  dtype (bf16/f16/f32): of bias [n]
  * and residual [m, n] (both nullable) and out; residual may be out.  Nothing but out's m rows is written, besides the workspace. */
 void vra_w8a8_gemm(const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales, const void* bias, const void* residual, void* out,
                    void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream);
 /* the gate / up pair of a feed-forward block (mlp.rs:451-469): out[m, n] = round(silu(g) u), g and u two such products in f32; dtype bf16/f16 */
 void vra_w8a8_gate_up_silu(const int8_t* x, const float* x_scales, const int8_t* w_gate, const float* s_gate, const int8_t* w_up, const float* s_up,
                            void* out, void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream);
+/* the kernel that they take for a product (its rows, and those of w, on multiples of 16 bytes where k is one), as slices of K << 16 | kind << 8 | size: kind 0 any alignment,
+ * 1 few rows (size: 16-column blocks of a workgroup, gate and up counted), 2 tiles (size: rows / 64 * 16 + columns / 64); 0: a shape they refuse */
+int32_t vra_w8a8_kernel(int32_t pair, int32_t m, int32_t k, int32_t n, int32_t has_workspace);
+/* the same products (w_up null: a single one) on a named kernel; the kernel changes no bit of the result */
+void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales, const int8_t* w_up, const float* s_up,
+                      const void* bias, const void* residual, void* out, void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype,
+                      int64_t stream);
 /* `workspace` of both: this many bytes on a multiple of 16, zeroed ONCE by the caller, one per concurrent stream (a captured graph counts as the stream it is replayed
  * on); products of few rows split K over workgroups that meet in it.  Null: no such split; the results are the same bits either way. */
 size_t vra_w8a8_workspace_bytes(void);

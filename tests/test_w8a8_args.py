@@ -44,7 +44,7 @@ def test_products():
 
     for name in ("x", "xs", "w", "ws", "out"):
         assert "null" in gemm(**{name: None})
-    for bad in (dict(m=-1), dict(k=0), dict(n=0), dict(k=131072)):
+    for bad in (dict(m=-1), dict(k=0), dict(n=0), dict(k=131072), dict(n=(1 << 24) + 1)):
         assert "131071" in gemm(**bad)
     assert "dtype" in gemm(dt=3)
     for bad in (dict(xs=P + 2), dict(ws=P + 1), dict(bias=P + 1), dict(residual=P + 1), dict(out=P + 1), dict(out=P + 2, dt=F32), dict(bias=P + 2, dt=F32)):
@@ -70,3 +70,39 @@ def test_no_rows_is_no_work():
 
 def test_workspace_size():
     assert ops.lib().vra_w8a8_workspace_bytes() >= 16
+
+
+def code(kind, size, slices=1):
+    return slices << 16 | kind << 8 | size
+
+
+def test_named_kernels():
+    def on(kernel, pair=False, x=P, bias=None, work=None, m=40, k=1024, n=512):
+        return refused("vra_w8a8_gemm_on", kernel, x, P, P, P, P if pair else None, P if pair else None, bias, None, P, work, m, k, n, BF16, 0)
+
+    for bad in (code(0, 1), code(0, 0, 2), code(3, 0), code(1, 3), code(1, 8), code(1, 4, 3), code(2, 0x11), code(2, 0x44, 2), code(2, 0x12, 16), -1, 0):
+        assert "no such kernel" in on(bad, work=P)
+    assert "no such kernel" in on(code(1, 1, 2))  # slices without a workspace
+    assert "no such kernel" in on(code(1, 1), m=65) and "no such kernel" in on(code(1, 4), m=33)
+    assert "no such kernel" in on(code(1, 1), pair=True) and "no such kernel" in on(code(0, 0), pair=True, bias=P)
+    assert "no such kernel" in on(code(2, 0x22), k=1000) and "no such kernel" in on(code(2, 0x22), x=P + 4) and "no such kernel" in on(code(1, 2), k=1000)
+    assert "no such kernel" in on(code(1, 1, 8), work=P, k=1008)  # runs without a step
+    assert "no such kernel" in on(code(2, 0x12, 2), work=P, m=8192, n=8192)  # more tiles than the workspace has counters for
+    assert "null" in on(code(0, 0), x=None)
+
+
+def test_kernel_choice():
+    pick = lambda pair, m, k, n, ws=1: _lib.load().vra_w8a8_kernel(pair, m, k, n, ws)
+    kind = lambda c: c >> 8 & 255
+    assert pick(0, 0, 64, 64) == 0 and pick(0, 1, 131072, 64) == 0 and pick(1, 5, 64, 0) == 0
+    for m in (1, 4, 16, 17, 64, 65, 150, 1021, 8192):
+        for k, n in ((4096, 6144), (14336, 4096), (3584, 32000), (128, 64), (16, 1), (1000, 300)):
+            for pair in (0, 1):
+                c, alone = pick(pair, m, k, n), pick(pair, m, k, n, 0)
+                assert alone >> 16 == 1 and c >> 16 in (1, 2, 4, 8)
+                if k % 16:
+                    assert kind(c) == (1 if m <= 64 else 0)
+                else:
+                    assert kind(c) == (1 if m <= 16 else 2 if m > 64 else kind(c))
+    assert pick(0, 8192, 14336, 4096) == code(2, 0x44) and pick(0, 1, 14336, 4096) == code(1, 1) and pick(0, 16, 3584, 32000) == code(1, 4)
+    assert pick(0, 64, 14336, 4096) >> 16 == 8 and pick(0, 64, 14336, 4096, 0) >> 16 == 1

@@ -109,6 +109,8 @@ def load():
     _sig(lib, "vra_add_rms_norm_i8", None, P, P, P, P, P, P, c_i32, c_i32, c_f32, c_i32, c_i64)
     _sig(lib, "vra_w8a8_gemm", None, P, P, P, P, P, P, P, P, c_i32, c_i32, c_i32, c_i32, c_i64)
     _sig(lib, "vra_w8a8_gate_up_silu", None, P, P, P, P, P, P, P, P, c_i32, c_i32, c_i32, c_i32, c_i64)
+    _sig(lib, "vra_w8a8_kernel", c_i32, c_i32, c_i32, c_i32, c_i32, c_i32)
+    _sig(lib, "vra_w8a8_gemm_on", None, c_i32, P, P, P, P, P, P, P, P, P, P, c_i32, c_i32, c_i32, c_i32, c_i64)
     _sig(lib, "vra_w8a8_workspace_bytes", c_sz)
     _sig(lib, "vra_rms_norm", None, P, P, P, c_i32, c_i32, c_f32, c_i32, c_i64)
     _sig(lib, "vra_qk_rms_norm", None, P, P, P, P, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32, c_i32, c_i64)

@@ -5,7 +5,9 @@
 // Weights = A, rows of x = B of v_mfma_i32_16x16x64_i8 (16 bytes of a row a lane; a lane's result: 4 consecutive columns of one row), at the bf16 instruction's
 // clocks for twice the K: every byte of an operand costs what it costs the 16-bit kernels (gemm_rows.cuh).
 #pragma once
-#include "common.cuh"
+#include <type_traits>
+
+#include "gemm_rows.cuh"
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a1 __attribute__((aligned(1)));  // 16 bytes anywhere
@@ -80,45 +82,155 @@ __device__ __forceinline__ void store4<PlainF32>(const float (&f)[4], void* p, s
       if (n + e < N) h[e] = f[e];
 }
 
+// an element as it is stored, and its value
+__device__ __forceinline__ uint32_t load1(int dtype, const void* p, size_t at) {
+  return dtype == VRA_F32 ? static_cast<const uint32_t*>(p)[at] : static_cast<const uint16_t*>(p)[at];
+}
+__device__ __forceinline__ float value1(int dtype, uint32_t v) {
+  return dtype == VRA_F32 ? __uint_as_float(v) : dtype == VRA_BF16 ? BF16::to_f32((uint16_t)v) : F16::to_f32((uint16_t)v);
+}
+__device__ __forceinline__ void store1(int dtype, float v, void* p, size_t at) {
+  if (dtype == VRA_F32) static_cast<float*>(p)[at] = v;
+  else static_cast<uint16_t*>(p)[at] = dtype == VRA_BF16 ? BF16::from_f32(v) : F16::from_f32(v);
+}
+
 // whether four columns at a multiple of 4 may be read and written at once, in all rows
 __host__ __device__ __forceinline__ bool i8_whole_fours(const GemmI8Args& a) {
   const uintptr_t all = (uintptr_t)a.out | (uintptr_t)a.residual | (uintptr_t)a.bias;
   return a.N % 4 == 0 && all % (a.dtype == VRA_F32 ? 16 : 8) == 0;
 }
 
-// sums g (and u) of columns n .. n + 3 of row m -> what is stored there
+// what stands behind the sums g (and u) of an element
 template <bool PAIR>
-__device__ __forceinline__ void i8_values(const GemmI8Args& a, float xs, int n, i32x4 g, i32x4 u, float (&y)[4]) {
+__device__ __forceinline__ float i8_value(int g, int u, float xs, float gs, float us) {
+  float v = (float)g * xs * gs;
+  if (PAIR) {
+    // silu(v) u = v u / (1 + exp(-v)); below zero exp(v / 2) goes to both factors: exp(-v) would end at v = -88, where bf16 still holds the result.  The hardware's
+    // exp2 and reciprocal, a step each and |v| / 2 steps by the exponent's rounding: a 16-bit result's own rounding is 2^12 (f16) and 2^15 times as coarse
+    const float h = __builtin_amdgcn_exp2f(-0.72134752f * fabsf(v)), s = v < 0.f ? h : 1.0f;
+    v = v * s * __builtin_amdgcn_rcpf(fmaf(h, h, 1.0f)) * ((float)u * xs * us * s);
+  }
+  asm("" : "+v"(v));  // (the last product is not drawn into a conversion to f16, here or there: the bits are the same in all kernels)
+  return v;
+}
+// what the epilogue reads of four columns n .. n + 3: the same for all rows
+struct I8Columns {
+  float g[4], u[4], bias[4];
+};
+template <class T, bool PAIR>
+__device__ __forceinline__ I8Columns i8_columns(const GemmI8Args& a, int n, bool whole) {
+  I8Columns c = {};
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    const int c = min(n + e, a.N - 1);
-    float v = (float)g[e] * xs * a.ws[0][c];
-    if (PAIR) {
-      // silu(v) u = v u / (1 + exp(-v)); below zero exp(v / 2) goes to both factors: exp(-v) would end at v = -88, where bf16 still holds the result
-      const float h = expf(-0.5f * fabsf(v)), s = v < 0.f ? h : 1.0f;
-      v = v * s / (1.0f + h * h) * ((float)u[e] * xs * a.ws[1][c] * s);
-    }
-    y[e] = v;
+    const int at = min(n + e, a.N - 1);
+    c.g[e] = a.ws[0][at];
+    if (PAIR) c.u[e] = a.ws[1][at];
   }
+  if (!PAIR && a.bias && n < a.N) load4<T>(c.bias, a.bias, n, n, a.N, whole && n + 4 <= a.N);
+  return c;
 }
+// sums g (and u) of columns n .. n + 3 of row m
 template <class T, bool PAIR>
-__device__ __forceinline__ void i8_store(const GemmI8Args& a, int m, int n, bool whole, i32x4 g, i32x4 u) {
+__device__ __forceinline__ void i8_store(const GemmI8Args& a, const I8Columns& c, float xs, int m, int n, bool whole, i32x4 g, i32x4 u) {
   if (m >= a.M || n >= a.N) return;
   whole = whole && n + 4 <= a.N;
   const size_t at = (size_t)m * a.N + n;
   float y[4], f[4];
-  i8_values<PAIR>(a, a.xs[m], n, g, u, y);
-  if (!PAIR && a.bias) {
-    load4<T>(f, a.bias, n, n, a.N, whole);
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] += f[e];
-  }
-  if (!PAIR && a.residual) {
-    load4<T>(f, a.residual, at, n, a.N, whole);
+  for (int e = 0; e < 4; e++) y[e] = i8_value<PAIR>(g[e], u[e], xs, c.g[e], c.u[e]);
+  if (!PAIR) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] += f[e];
+    for (int e = 0; e < 4; e++) y[e] += c.bias[e];
+    if (a.residual) {
+      load4<T>(f, a.residual, at, n, a.N, whole);
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] += f[e];
+    }
   }
   store4<T>(y, a.out, at, n, a.N, whole);
+}
+
+// whether eight columns at a multiple of 8 (f32: four at a multiple of 4) are 16 bytes on their place, in all rows
+__host__ __device__ __forceinline__ bool i8_sixteens(const GemmI8Args& a) {
+  return a.N % (a.dtype == VRA_F32 ? 4 : 8) == 0 && ((uintptr_t)a.out | (uintptr_t)a.residual | (uintptr_t)a.bias) % 16 == 0;
+}
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
+// A wave's R blocks of 16 rows x 64 virtual columns (acc[block][tile of 16 columns]) for i8_sixteens: lane (r16, q4) holds columns 4 q4 .. + 3 of the tiles, of row r16 of the
+// blocks.  m: that row in block 0; n0: the wave's first column.  What is read of rows and columns is asked for together, the residual two blocks ahead (one
+// after the other, they were 30 of a 256 x 256 tile's 39 us behind its loop); 16-bit results trade places between a row's four lanes and go out 16 bytes a lane.
+template <class T, bool PAIR, int R>
+__device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0, int q4, const i32x4 (&acc)[R][4]) {
+  constexpr int NJ = PAIR ? 2 : 4;
+  constexpr bool F32 = std::is_same<T, PlainF32>::value;
+  typedef typename std::conditional<F32, f32x4, u32x2>::type Four;
+  const int M = a.M, N = a.N;
+  float gs[NJ][4], us[NJ][4], xs[R];
+  Four bias[NJ], res[2][NJ];
+  auto fetch = [&](int i) {
+    const size_t row = (size_t)min(m + i * 16, M - 1) * N;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const size_t at = row + min(n0 + j * 16 + q4 * 4, N - 4);
+      if constexpr (F32) res[i & 1][j] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.residual) + at);
+      else res[i & 1][j] = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.residual) + at);
+    }
+  };
+  const bool has_res = !PAIR && a.residual, has_bias = !PAIR && a.bias;
+  if (has_res) {
+    fetch(0);
+    if (R > 1) fetch(1);
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; j++) {
+    const int n = min(n0 + j * 16 + q4 * 4, N - 4);
+    const f32x4 g = *reinterpret_cast<const f32x4_a4*>(a.ws[0] + n), u = PAIR ? (f32x4)*reinterpret_cast<const f32x4_a4*>(a.ws[1] + n) : g;
+#pragma unroll
+    for (int e = 0; e < 4; e++) gs[j][e] = g[e], us[j][e] = u[e];
+    if (has_bias) {
+      if constexpr (F32) bias[j] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.bias) + n);
+      else bias[j] = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.bias) + n);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; i++) xs[i] = a.xs[min(m + i * 16, M - 1)];
+  auto add = [&](float (&y)[4], const Four& v) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if constexpr (F32) y[e] += v[e];
+      else y[e] += T::to_f32((uint16_t)(v[e >> 1] >> (e & 1 ? 16 : 0)));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    float y[NJ][4];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[j][e] = i8_value<PAIR>(acc[i][PAIR ? 2 * j : j][e], acc[i][PAIR ? 2 * j + 1 : j][e], xs[i], gs[j][e], us[j][e]);
+      if (has_bias) add(y[j], bias[j]);
+      if (has_res) add(y[j], res[i & 1][j]);
+    }
+    if (has_res && i + 2 < R) fetch(i + 2);
+    const bool in = m + i * 16 < M;
+    const size_t row = (size_t)(m + i * 16) * N;
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        const int n = n0 + j * 16 + q4 * 4;
+        if (in && n < N) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + row + n) = f32x4{y[j][0], y[j][1], y[j][2], y[j][3]};
+      }
+    } else {
+      u32x2 v[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; j++) v[j] = u32x2{T::pack2(y[j][0], y[j][1]), T::pack2(y[j][2], y[j][3])};
+      gr_gather_columns(v);
+#pragma unroll
+      for (int h = 0; h < NJ / 2; h++) {
+        const int n = n0 + q4 * (NJ * 4) + h * 8;
+        if (in && n < N) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + row + n) = u32x4{v[2 * h][0], v[2 * h][1], v[2 * h + 1][0], v[2 * h + 1][1]};
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------- any K, any alignment
@@ -174,12 +286,416 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(const GemmI8Args a, in
   VRA_MFMA_DRAIN();
   const bool whole = i8_whole_fours(a);
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int m = m0 + xr + i * 16 + r16;
-    if (PAIR) i8_store<T, true>(a, m, n0 + (wr >> 1) + q4 * 4, whole, acc[i][0], acc[i][1]);
-    else
+  for (int j = 0; j < (PAIR ? 1 : 2); j++) {
+    const int n = n0 + (PAIR ? wr >> 1 : wr + j * 16) + q4 * 4;
+    const I8Columns c = i8_columns<T, PAIR>(a, n, whole);
 #pragma unroll
-      for (int j = 0; j < 2; j++) i8_store<T, false>(a, m, n0 + wr + j * 16 + q4 * 4, whole, acc[i][j], acc[i][j]);
+    for (int i = 0; i < 2; i++) {
+      const int m = m0 + xr + i * 16 + r16;
+      i8_store<T, PAIR>(a, c, a.xs[min(m, a.M - 1)], m, n, whole, acc[i][j], acc[i][1]);
+    }
   }
+#endif
+}
+
+// ---------------------------------------------------------------- few rows (decode)
+// Where the K slices of a product meet: a partial tile of every slice but the last to arrive, and a counter a tile (a line each), zero between calls.
+#define I8_WS_COUNTERS 1024
+#define I8_WS_PARTIALS ((size_t)I8_WS_COUNTERS * 64)
+#define I8_WS_PARTIAL_BYTES ((size_t)32 << 20)
+#define I8_WS_BYTES (I8_WS_PARTIALS + I8_WS_PARTIAL_BYTES)
+
+// Stores `n` sums a thread (v) of slice `z` of a tile and returns whether this workgroup is the tile's last: then the other slices' sums have been added to v, and the counter
+// is zero again.  All threads call it; `flag`: a word of LDS that nobody reads or writes by other means any more.  Nobody waits for anybody.  Sums go through memory with agent scope (sc1: the L2s of the XCDs are not
+// coherent), each store is acknowledged before its workgroup counts itself, and the last one reads behind all counts.
+template <int V, int THREADS>
+__device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int tiles, int z, int slices, int* flag) {
+  const int tid = threadIdx.x;
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(static_cast<char*>(ws) + I8_WS_PARTIALS, 0, 0x7FFFFFF0, 0x00020000u);
+  constexpr int W = V % 4 ? 1 : 4;  // sums a store
+  auto at = [&](int s, int i) { return (uint32_t)(((s * tiles + tile) * (V / W) + i) * THREADS + tid) * (4u * W); };
+#pragma unroll
+  for (int i = 0; i < V / W; i++) {
+    if constexpr (W == 4) __builtin_amdgcn_raw_buffer_store_b128(u32x4{(uint32_t)v[4 * i], (uint32_t)v[4 * i + 1], (uint32_t)v[4 * i + 2], (uint32_t)v[4 * i + 3]}, r, at(z, i), 0, 16);
+    else __builtin_amdgcn_raw_buffer_store_b32((uint32_t)v[i], r, at(z, i), 0, 16);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  uint32_t* const count = static_cast<uint32_t*>(ws) + tile * 16;
+  if (tid == 0) *flag = (int)__hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == slices - 1;
+  __syncthreads();
+  if (!*flag) return false;
+  for (int s = 0; s < slices; s++) {
+    if (s == z) continue;
+    if constexpr (W == 4) {
+      u32x4 p[V / 4];
+#pragma unroll
+      for (int i = 0; i < V / 4; i++) p[i] = __builtin_amdgcn_raw_buffer_load_b128(r, at(s, i), 0, 16);
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] += (int)p[i >> 2][i & 3];
+    } else {
+      uint32_t p[V];
+#pragma unroll
+      for (int i = 0; i < V; i++) p[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at(s, i), 0, 16);
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] += (int)p[i];
+    }
+  }
+  if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
+}
+
+#define I8_NW 8
+// Bound: the weights' way through memory.  A workgroup takes 16 C virtual columns (pair: gate and up blocks of 16 in turn), all MT 16 rows and one of `slices` runs of
+// K; its eight waves take the run's steps of 128 in turn, straight into registers, U of them asked for at once (a lane: 32 bytes of its row, so that a wave's request covers whole
+// lines).  The waves' sums meet in LDS, the slices' in the workspace.  ANY: rows that begin anywhere, or K off 16.
+template <bool PAIR, int MT, int C, int U, bool ANY>
+__global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Args a, void* ws, int slices) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int NW = I8_NW;
+  constexpr int CO = PAIR ? C / 2 : C, OUT = MT * CO * 256, E = (OUT + NW * 64 - 1) / (NW * 64);  // results of the workgroup, of a thread
+  __shared__ __attribute__((aligned(16))) int part[NW * MT * C * 256];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int M = a.M, N = a.N, K = a.K, tile = (int)blockIdx.x / slices, z = (int)blockIdx.x - tile * slices, n0 = tile * CO * 16;
+  const int8_t* wp[C];
+  const int8_t* xp[MT];
+#pragma unroll
+  for (int c = 0; c < C; c++) wp[c] = (PAIR && (c & 1) ? a.w[1] : a.w[0]) + (size_t)min(n0 + (PAIR ? c >> 1 : c) * 16 + r16, N - 1) * K + q4 * 32;
+#pragma unroll
+  for (int i = 0; i < MT; i++) xp[i] = a.x + (size_t)min(i * 16 + r16, M - 1) * K + q4 * 32;
+  u32x4 w[U][C][2], x[U][MT][2];
+  auto load = [&](int u, int step) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int at = step * 128 + h * 16;
+#pragma unroll
+      for (int c = 0; c < C; c++) w[u][c][h] = ANY ? (u32x4)*reinterpret_cast<const u32x4_a1*>(wp[c] + at) : *reinterpret_cast<const u32x4*>(wp[c] + at);
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+        if (i * 16 + r16 < M) x[u][i][h] = ANY ? (u32x4)*reinterpret_cast<const u32x4_a1*>(xp[i] + at) : *reinterpret_cast<const u32x4*>(xp[i] + at);
+    }
+  };
+  i32x4 acc[MT][C];
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int c = 0; c < C; c++) acc[i][c] = zero_acc_i8();
+  auto product = [&](int u) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int c = 0; c < C; c++) mfma_i8(acc[i][c], w[u][c][h], x[u][i][h]);
+  };
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int i = 0; i < MT; i++) x[u][i][0] = x[u][i][1] = u32x4{0u, 0u, 0u, 0u};  // (rows beyond M)
+  // the epilogue's operands: element o of the workgroup is column o % 4 + 4 (o / 64 % 4) of block o / 256 % CO, row o / 4 % 16 of block o / (256 CO)
+  float xs[E], gs[E], us[E];
+  uint32_t bias[E], res[E];
+  size_t at[E];
+  bool in[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int o = tid + e * NW * 64, l = o >> 2 & 63, m = o / (256 * CO) * 16 + (l & 15), n = n0 + (o >> 8) % CO * 16 + (l >> 4) * 4 + (o & 3);
+    in[e] = o < OUT && m < M && n < N;
+    at[e] = (size_t)m * N + n;
+    xs[e] = gs[e] = us[e] = 0.f, bias[e] = res[e] = 0u;
+    if (!in[e]) continue;
+    xs[e] = a.xs[m], gs[e] = a.ws[0][n];
+    if (PAIR) us[e] = a.ws[1][n];
+    if (!PAIR && a.bias) bias[e] = load1(a.dtype, a.bias, n);
+    if (!PAIR && a.residual) res[e] = load1(a.dtype, a.residual, at[e]);
+  }
+  // steps of 128 of the run, begun at another place in every workgroup: rows of a power of two bytes lie on the same channels of the memory, and all workgroups would ask for the same
+  // of them at a time (pair 1 x 14336, K = 4096, in order / so: 24.9 / 22.0 us; K = 3584: no difference)
+  const int whole = K >> 7, s0 = (int)((int64_t)whole * z / slices), len = (int)((int64_t)whole * (z + 1) / slices) - s0, turn = len ? tile * 5 % len : 0;
+  auto place = [&](int s) { return s0 + (s + turn < len ? s + turn : s + turn - len); };
+  for (int s = wave; s < len; s += NW * U) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (s + u * NW < len) load(u, place(s + u * NW));
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (s + u * NW < len) product(u);
+  }
+  if ((K & 127) && z == slices - 1 && wave == whole % NW) {  // what K leaves behind whole steps; a chunk beyond it counts nothing, as its x is zero
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int k = whole * 128 + q4 * 32 + h * 16, at = whole * 128 + h * 16, left = K - k;
+      auto take = [&](const int8_t* p) {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (left >= 16) v = ANY ? (u32x4)*reinterpret_cast<const u32x4_a1*>(p + at) : *reinterpret_cast<const u32x4*>(p + at);
+        else if (ANY)
+#pragma unroll
+          for (int e = 0; e < 15; e++)
+            if (e < left) v[e >> 2] |= (uint32_t)(uint8_t)p[at + e] << (8 * (e & 3));
+        return v;
+      };
+#pragma unroll
+      for (int c = 0; c < C; c++) w[0][c][h] = take(wp[c]);
+#pragma unroll
+      for (int i = 0; i < MT; i++) x[0][i][h] = take(xp[i]);
+    }
+    product(0);
+  }
+  VRA_MFMA_DRAIN();
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int c = 0; c < C; c++) *reinterpret_cast<i32x4*>(&part[((wave * MT + i) * C + c) * 256 + lane * 4]) = acc[i][c];
+  __syncthreads();
+  int sums[E * (PAIR ? 2 : 1)];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int o = tid + e * NW * 64, b = o >> 8;  // block (i, column block) of the results; its sums are in blocks of C a row block
+    const int* p = &part[(PAIR ? b * 2 : b) * 256 + (o & 255)];
+    int g = 0, u = 0;
+    if (o < OUT)
+#pragma unroll
+      for (int v = 0; v < NW; v++) {
+        g += p[v * MT * C * 256];
+        if (PAIR) u += p[v * MT * C * 256 + 256];
+      }
+    sums[e] = g;
+    if (PAIR) sums[E + e] = u;
+  }
+  if (slices > 1 && !i8_meet<E * (PAIR ? 2 : 1), NW * 64>(sums, ws, tile, (int)gridDim.x / slices, z, slices, part)) return;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if (!in[e]) continue;
+    float y = i8_value<PAIR>(sums[e], PAIR ? sums[E + e] : 0, xs[e], gs[e], us[e]);
+    if (!PAIR) y = y + value1(a.dtype, bias[e]) + value1(a.dtype, res[e]);
+    store1(a.dtype, y, a.out, at[e]);
+  }
+#endif
+}
+
+// ---------------------------------------------------------------- many rows (prompts, larger batches)
+// The loop, the two groups of waves and the LDS layout of gemm_rows.cuh, whose K step of 64 16-bit elements is 128 bytes of a row as one of 128 here is: the same requests,
+// LDS reads and clocks, twice the products.  Bound: as there, the chip's power at 256 x 256, what a CU gets past L2 below it.
+// K any multiple of 16: in the last step a chunk of x beyond K is taken as zeros, so what stands in its place of w (the next row's bytes) counts nothing; the
+// tensors' descriptors end with their last row, nothing behind it is read.
+// slices > 1: a tile's K steps in as many runs, a workgroup each, that meet in the workspace (i8_meet).
+struct GemmI8Tiles {
+  void* ws;
+  int MT, NT, slices;
+};
+
+// PAIR: virtual columns, gate and up interleaved in blocks of 16
+template <bool PAIR, int BM, int BN, bool DEEP>
+__global__ __launch_bounds__(512, 2) void gemm_i8_tile_kernel(const GemmI8Args a, const GemmI8Tiles g) {
+#ifdef __HIP_DEVICE_COMPILE__
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  using G = GrTile<BM, BN, DEEP>;
+  constexpr int H = G::H, KP = G::KP, S = G::S, NX = G::NX, STG = G::STG, EX = G::EX, EW = G::EW, D = EX + EW;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wg = wave >> 2, cw = (wave & 3) % G::CW, rw = (wave & 3) / G::CW, r16 = lane & 15, q4 = lane >> 4;
+  // the tile and its run of K steps.  slices (1, 2, 4, 8): a place of K belongs to 8 / slices XCDs (ids mod 8), which read that part of x and w only; within it contiguous runs of
+  // the tiles' order go to one XCD each
+  const int tiles = g.MT * g.NT, z = (int)blockIdx.x % g.slices, id = (int)blockIdx.x / g.slices, P = 8 / g.slices, q = tiles / P, r = tiles % P, p = id % P;
+  const int lin = p * q + min(p, r) + id / P;
+  int mt, nt;
+  gr_tile_of(lin, g.MT, g.NT, mt, nt);
+  const int K = a.K, KT = (K + 127) >> 7, ks0 = (int)((int64_t)KT * z / g.slices), ks1 = (int)((int64_t)KT * (z + 1) / g.slices);
+  const int m0 = mt * BM, n0 = nt * (PAIR ? BN / 2 : BN), rows = min(a.M - m0, BM), cols = min(a.N - n0, PAIR ? BN / 2 : BN);  // (n0: of each tensor)
+  const int8_t* const x = a.x + (size_t)m0 * K;
+  const int8_t* const w0 = a.w[0] + (size_t)n0 * K;
+  const int8_t* const w1 = PAIR ? a.w[1] + (size_t)n0 * K : w0;
+  // (pair: virtual block f is of tensor f & 1.  A wave requests the blocks 2 wave and 2 wave + 1 of a 256-column tile, block wave of a 128-column one)
+  const int8_t* const wlo = PAIR && EW == 2 && (wave & 1) ? w1 : w0;
+  const int8_t* const whi = PAIR && EW == 4 ? w1 : wlo;
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(x), 0, rows * K, 0x00020000u);
+  const __amdgpu_buffer_rsrc_t rlo = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wlo), 0, cols * K, 0x00020000u);
+  const __amdgpu_buffer_rsrc_t rhi = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(whi), 0, cols * K, 0x00020000u);
+  const int sr = lane >> 3, sc = (lane & 7) ^ sr;
+  auto upper = [&](int e) { return EX == 4 ? e < 2 : e == 0 || (e == 1 && wave < 4); };
+  auto xrow8 = [&](int e) {
+    if (H == 1) return (wave * EX + e) * 8;
+    if (EX == 4) return (wave < 4 ? wave : wave + 4) * 16 + (e >> 1) * 64 + (e & 1) * 8;
+    const int i = wave < 4 ? (upper(e) ? wave * 2 + e : 8 + wave) : (upper(e) ? 4 + wave : (wave - 4) * 2 + e - 1);
+    return i / 6 * 96 + i % 6 * 8 + (upper(e) ? 0 : 48);
+  };
+  uint32_t vx[EX], vw[EW];
+#pragma unroll
+  for (int e = 0; e < EX; e++) vx[e] = (uint32_t)min(xrow8(e) + sr, rows - 1) * (uint32_t)K + (uint32_t)sc * 16u;
+#pragma unroll
+  for (int e = 0; e < EW; e++) {
+    const int r8 = (wave * EW + e) * 8;
+    vw[e] = (uint32_t)min((PAIR ? (r8 >> 5) * 16 + (r8 & 15) : r8) + sr, cols - 1) * (uint32_t)K + (uint32_t)sc * 16u;
+  }
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  // requests of K step ks (beyond the run: its last step again, never read) into the buffer at byte `o`
+  auto stage_x = [&](int o, int ks, int e0, int e1) {
+    const uint32_t so = (uint32_t)min(ks, ks1 - 1) * 128u;
+#pragma unroll
+    for (int e = e0; e < e1; e++) __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(smem + o + xrow8(e) * 128), 16, vx[e], so, 0, 0);
+  };
+  auto stage_half = [&](int o, int ks, bool up) {
+#pragma unroll
+    for (int e = 0; e < EX; e++)
+      if (upper(e) == up) stage_x(o, ks, e, e + 1);
+  };
+  auto stage_w = [&](int o, int ks) {
+    const uint32_t so = (uint32_t)min(ks, ks1 - 1) * 128u;
+#pragma unroll
+    for (int e = 0; e < EW; e++) {
+      unsigned char* const d = smem + o + G::XB * 2048 + (wave * EW + e) * 1024;
+      if (e < EW / 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(rlo, (lds_ptr)d, 16, vw[e], so, 0, 0);
+      else __builtin_amdgcn_raw_ptr_buffer_load_lds(rhi, (lds_ptr)d, 16, vw[e], so, 0, 0);
+    }
+  };
+  const int row0 = wg * (BM / 2) + rw * (BM / 2 / G::RW);  // the wave's first row in the tile
+  const int c0 = r16 * 128 + (q4 ^ (r16 & 7)) * 16, c1 = c0 ^ 64;
+  const unsigned char* const xb = smem + row0 * 128;
+  const unsigned char* const wb = smem + G::XB * 2048 + cw * 4 * 2048;
+  u32x4 xa[KP * NX][2], wa[KP * 4][2];
+  auto read_x = [&](int o, int h, int k = 0) {
+#pragma unroll
+    for (int i = 0; i < NX; i++) {
+      xa[k * NX + i][0] = *reinterpret_cast<const u32x4*>(xb + o + c0 + (h * NX + i) * 2048);
+      xa[k * NX + i][1] = *reinterpret_cast<const u32x4*>(xb + o + c1 + (h * NX + i) * 2048);
+    }
+  };
+  auto read_w = [&](int o, int k = 0) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      wa[k * 4 + j][0] = *reinterpret_cast<const u32x4*>(wb + o + c0 + j * 2048);
+      wa[k * 4 + j][1] = *reinterpret_cast<const u32x4*>(wb + o + c1 + j * 2048);
+    }
+  };
+  i32x4 acc[H * NX][4];
+#pragma unroll
+  for (int i = 0; i < H * NX; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = zero_acc_i8();
+  // (a wave's 64 columns, a phase's rows: nothing of them in the matrix, no MFMAs)
+  const bool in_c = (PAIR ? cw * 32 : cw * 64) < cols, in = in_c && row0 < rows, in1 = H == 2 && in_c && row0 + NX * 16 < rows;
+  auto compute = [&](auto HH, int ks) {  // K steps ks .. ks + KP - 1, those of them within the run
+    constexpr int h = decltype(HH)::value;
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(H == 2 ? D : (S - 2) * KP * D) : "memory");
+#pragma unroll
+    for (int k = 0; k < KP; k++)
+      if ((ks + k) * 128 + 128 > K) {  // (the last step of a K off 128, or an H = 2 step behind an odd number of them)
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++) {
+          const bool beyond = (ks + k) * 128 + kc * 64 + q4 * 16 >= K;
+#pragma unroll
+          for (int i = 0; i < NX; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) xa[k * NX + i][kc][e] = beyond ? 0u : xa[k * NX + i][kc][e];
+        }
+        asm volatile("s_nop 1");
+      }
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (h ? in1 : in) {
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int k = 0; k < KP; k++) {
+        if (k && ks + k >= ks1) break;
+#pragma unroll
+        for (int kc = 0; kc < 2; kc++)
+#pragma unroll
+          for (int i = 0; i < NX; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) mfma_i8_ready(acc[h * NX + i][j], wa[k * 4 + j][kc], xa[k * NX + i][kc]);
+      }
+      __builtin_amdgcn_s_setprio(0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+  };
+  auto no_scalar_loads = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using C0 = std::integral_constant<int, 0>;
+  using C1 = std::integral_constant<int, 1>;
+  if constexpr (H == 2) {
+    stage_half(0, 0, true);
+    stage_w(0, 0);
+    stage_half(0, 0, false);
+    stage_half(STG, 1, true);
+    stage_w(STG, 1);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D) : "memory");
+    __builtin_amdgcn_s_barrier();
+    if (wg == 1) __builtin_amdgcn_s_barrier();  // the second group runs one barrier behind the first
+    auto step = [&](auto B, int ks) {
+      constexpr int o = decltype(B)::value * STG;
+      read_w(o);
+      __builtin_amdgcn_sched_barrier(0);
+      read_x(o, 0);
+      stage_half(STG - o, ks + 1, false);
+      compute(C0{}, ks);
+      read_x(o, 1);
+      stage_half(o, ks + 2, true);
+      stage_w(o, ks + 2);
+      compute(C1{}, ks);
+    };
+    no_scalar_loads();
+    for (int ks = 0; ks < KT; ks += 2) {
+      step(C0{}, ks);
+      step(C1{}, ks + 1);
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < (S - 1) * KP; s++) stage_x(s * STG, ks0 + s, 0, EX), stage_w(s * STG, ks0 + s);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * KP * D) : "memory");
+    __builtin_amdgcn_s_barrier();
+    if (wg == 1) __builtin_amdgcn_s_barrier();
+    no_scalar_loads();
+    int o = 0, p = (S - 1) * KP * STG;  // buffers of this phase and of the one before it
+    for (int ks = ks0; ks < ks1; ks += KP) {
+#pragma unroll
+      for (int k = 0; k < KP; k++) read_w(o + k * STG, k), read_x(o + k * STG, 0, k);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < KP; k++) {
+        stage_x(p + k * STG, ks + (S - 1) * KP + k, 0, EX);
+        stage_w(p + k * STG, ks + (S - 1) * KP + k);
+      }
+      compute(C0{}, ks);
+      p = o;
+      o = o == (S - 1) * KP * STG ? 0 : o + KP * STG;
+    }
+  }
+  if (wg == 0) __builtin_amdgcn_s_barrier();
+  // (the requests beyond the run still write LDS: they end before the workgroup does)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  VRA_MFMA_DRAIN();
+  if constexpr (H == 1) {
+    if (g.slices > 1) {
+      int v[NX * 16];
+#pragma unroll
+      for (int i = 0; i < NX * 16; i++) v[i] = acc[i >> 4][i >> 2 & 3][i & 3];
+      if (!i8_meet<NX * 16, 512>(v, g.ws, lin, tiles, z, g.slices, reinterpret_cast<int*>(smem))) return;
+#pragma unroll
+      for (int i = 0; i < NX * 16; i++) acc[i >> 4][i >> 2 & 3][i & 3] = v[i];
+    }
+  }
+  const bool sixteens = i8_sixteens(a), whole = i8_whole_fours(a);
+  auto finish = [&](auto t) {
+    using T = decltype(t);
+    if (sixteens) return i8_store_rows<T, PAIR, H * NX>(a, m0 + row0 + r16, n0 + (PAIR ? cw * 32 : cw * 64), q4, acc);
+#pragma unroll
+    for (int j = 0; j < (PAIR ? 2 : 4); j++) {
+      const int n = n0 + (PAIR ? cw * 32 : cw * 64) + j * 16 + q4 * 4;
+      const I8Columns c = i8_columns<T, PAIR>(a, n, whole);
+#pragma unroll
+      for (int i = 0; i < H * NX; i++) {
+        const int m = m0 + row0 + i * 16 + r16;
+        i8_store<T, PAIR>(a, c, a.xs[min(m, a.M - 1)], m, n, whole, acc[i][PAIR ? 2 * j : j], acc[i][PAIR ? 2 * j + 1 : j]);
+      }
+    }
+  };
+  if (a.dtype == VRA_BF16) finish(BF16{});
+  else if (PAIR || a.dtype == VRA_F16) finish(F16{});
+  else finish(PlainF32{});
 #endif
 }

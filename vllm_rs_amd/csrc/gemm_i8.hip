@@ -1,54 +1,174 @@
-// gemm_i8.hip — the C entry points of the 8-bit integer products (gemm_i8.cuh).
+// gemm_i8.hip — the C entry points of the 8-bit integer products (gemm_i8.cuh), and which kernel a product runs on.
 #include "gemm_i8.cuh"
 
 #include <algorithm>
 
 namespace {
 
-template <class F>
-void with_type(int dtype, const F& f) {
-  if (dtype == VRA_BF16) f(BF16{});
-  else if (dtype == VRA_F16) f(F16{});
-  else f(PlainF32{});
+// a kernel: kind << 8 | its size, and the slices of K << 16
+enum { I8_ANY = 0, I8_FEW = 1, I8_TILE = 2 };
+struct Choice {
+  int kind, size, slices;  // few: virtual columns / 16 of a workgroup; tile: rows / 64 * 16 + virtual columns / 64
+};
+
+// whether rows of x and w may be read 16 bytes at a time from where they begin
+bool in_sixteens(const GemmI8Args& a) { return ((uintptr_t)a.x | (uintptr_t)a.w[0] | (uintptr_t)a.w[1] | (uintptr_t)a.K) % 16 == 0; }
+
+int64_t over(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int64_t few_tiles(int N, bool pair, int C) { return over(N, pair ? C * 8 : C * 16); }
+bool few_has(bool pair, int M, int C) {
+  const int MT = (M + 15) / 16;
+  return pair ? (C == 2 && MT <= 4) || (C == 4 && MT <= 2) || (C == 8 && MT == 1) : (C == 1 || C == 2 ? MT <= 4 : C == 4 && MT <= 2);
+}
+int64_t tile_count(int M, int N, bool pair, int t) { return over(M, (t >> 4) * 64) * over(N, (t & 15) * (pair ? 32 : 64)); }
+bool tile_has(int t) { return t == 0x12 || t == 0x22 || t == 0x32 || t == 0x24 || t == 0x34 || t == 0x44; }
+// whether `slices` runs of K have a step each and meet within the workspace
+bool slices_fit(int slices, int K, int64_t tiles, int64_t tile_bytes) {
+  return slices == 1 || ((slices == 2 || slices == 4 || slices == 8) && slices <= K / 128 && tiles <= I8_WS_COUNTERS && tiles * slices * tile_bytes <= (int64_t)I8_WS_PARTIAL_BYTES);
+}
+int64_t few_bytes(bool pair, int M, int C) {  // of a workgroup's sums, in whole rounds of its threads
+  const int CO = pair ? C / 2 : C;
+  return over((int64_t)(M + 15) / 16 * CO * 256, I8_NW * 64) * I8_NW * 64 * 4 * (pair ? 2 : 1);
+}
+
+// Times in us, fitted to 2100 (few) and 2400 (tile) measured ones: 1..64 and 17..8192 rows, 15 products of K = 992..18944 and 512..32000 columns, weights from memory, rms 12 and 7..13 %; the
+// choice by them is 1.0 % behind the best one measured on average, 22 % at most (48 rows x 5632 + 5632, K = 2048).
+// few: what the busiest CU reads, at 35 GB/s, and what the chip reads, weights at 6.55 TB/s and the rows of x, once a workgroup, at 13.9; the longer of them and a quarter of the other
+double few_us(bool pair, int M, int N, int K, int C, int slices) {
+  const double wgs = (double)few_tiles(N, pair, C) * slices, t = pair ? 2 : 1;
+  const double cu = (double)over((int64_t)wgs, 256) * (16.0 * C + M) * K / slices / 34.9e3;
+  const double chip = t * N * K / 6.55e6 + wgs / slices * M * K / 13.9e6;
+  return 2.41 + (slices > 1 ? 0.82 + 0.50 * slices : 0.0) + std::max(cu, chip) + 0.245 * std::min(cu, chip);
+}
+// tile: as in gemm_rows_tile (gemm_rows.cuh): rounds of 256 workgroups (64 x 128 on few: two a CU), for each a fixed time and one for each K step, the last round's between that of few workgroups
+// and of all; and the slices' meeting.  Never quicker than the weights' way through memory.
+double tile_us(bool pair, int M, int N, int K, int t, int slices) {
+  const int64_t wgs = tile_count(M, N, pair, t) * slices;
+  const bool deep = t == 0x12 && wgs <= 256;
+  struct Times { int tile; double t0, round, one, half, full, meet, slice; };
+  static const Times times[7] = {{0x12, 2.7, 4.33, 0.421, 0.679, 0.695, 3.53, 0.99}, {0x22, 0.0, 5.79, 0.429, 0, 0.566, 0.77, 1.28}, {0x32, 2.2, 3.10, 0.560, 0, 0.762, 1.32, 1.65},
+                                 {0x24, 2.9, 2.86, 0.710, 0, 0.987, 2.22, 1.74}, {0x34, 0.6, 6.33, 0.803, 0, 1.121, 0, 0}, {0x44, 0.0, 8.24, 0.930, 0, 1.438, 0, 0},
+                                 {0x12, 0.8, 3.57, 0.363, 0, 0.493, 0.85, 0.79}};
+  const Times* c = &times[6];
+  if (!deep)
+    for (c = times; c->tile != t;) c++;
+  const int slots = t == 0x12 && !deep ? 512 : 256;
+  const double full = (double)(wgs / slots), rem = (double)(wgs % slots), steps = (double)over(K, 128) / slices;
+  double last = rem > 0 ? c->one + (c->full - c->one) * rem / slots : 0.0;
+  if (slots == 512 && rem > 0) last = rem <= 256 ? c->one : c->half + (c->full - c->half) * (rem - 256) / 256;
+  const double us = c->t0 + (full + (rem > 0)) * c->round + steps * (full * c->full + last) + (slices > 1 ? c->meet + c->slice * slices : 0.0);
+  return std::max(us, 3.0 + (pair ? 2.0 : 1.0) * N * K / 6.3e6);
+}
+
+Choice choose(bool pair, int M, int N, int K, bool workspace, bool sixteens) {
+  if (!sixteens) return M <= 64 ? Choice{I8_FEW, pair ? 2 : 1, 1} : Choice{I8_ANY, 0, 1};
+  Choice best = {I8_TILE, 0x12, 1};
+  double us = 0.0;
+  auto offer = [&](int kind, int size, int slices, double v) {
+    if (us == 0.0 || v < us) best = Choice{kind, size, slices}, us = v;
+  };
+  for (int slices = 1; slices <= (workspace ? 8 : 1); slices *= 2) {
+    if (M <= 64)
+      for (int C = 1; C <= 8; C *= 2)
+        if (few_has(pair, M, C) && slices_fit(slices, K, few_tiles(N, pair, C), few_bytes(pair, M, C))) offer(I8_FEW, C, slices, few_us(pair, M, N, K, C, slices));
+    if (M > 16)
+      for (const int t : {0x12, 0x22, 0x32, 0x24, 0x34, 0x44})
+        if (t <= 0x32 ? slices_fit(slices, K, tile_count(M, N, pair, t), (t >> 4) * (t & 15) * 16384) : slices == 1) offer(I8_TILE, t, slices, tile_us(pair, M, N, K, t, slices));
+  }
+  return best;
+}
+
+template <bool PAIR, int MT, int C, bool ANY>
+void few(const GemmI8Args& a, void* ws, int slices, hipStream_t st) {
+  // (one row block of 16 columns: two steps at once pay, as a wave has little else in flight: 1 x 4096, K = 14336 12.9 us, 14.6 without; 32 rows 25.3 / 22.0)
+  constexpr int U = MT == 1 && C == 1 ? 2 : 1;
+  gemm_i8_few_kernel<PAIR, MT, C, U, ANY><<<(unsigned)(few_tiles(a.N, PAIR, C) * slices), I8_NW * 64, 0, st>>>(a, ws, slices);
+}
+template <bool PAIR, int C, bool ANY>
+void few_rows(const GemmI8Args& a, void* ws, int slices, hipStream_t st) {
+  constexpr int most = C <= 2 ? 4 : C == 4 ? 2 : 1;  // (few_has)
+  if (a.M <= 16) return few<PAIR, 1, C, ANY>(a, ws, slices, st);
+  if constexpr (most >= 2)
+    if (a.M <= 32) return few<PAIR, 2, C, ANY>(a, ws, slices, st);
+  if constexpr (most >= 4) a.M <= 48 ? few<PAIR, 3, C, ANY>(a, ws, slices, st) : few<PAIR, 4, C, ANY>(a, ws, slices, st);
+}
+
+template <bool PAIR, int BM, int BN, bool DEEP>
+void tile(const GemmI8Args& a, void* ws, int slices, hipStream_t st) {
+  using G = GrTile<BM, BN, DEEP>;
+  constexpr int BC = PAIR ? BN / 2 : BN;
+  const GemmI8Tiles g = {ws, (a.M + BM - 1) / BM, (a.N + BC - 1) / BC, slices};
+  void (*const k)(GemmI8Args, GemmI8Tiles) = gemm_i8_tile_kernel<PAIR, BM, BN, DEEP>;
+  static uint64_t attr_devs = 0;  // function attributes belong to the device current at the call
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  if (!((__atomic_load_n(&attr_devs, __ATOMIC_RELAXED) >> (dev & 63)) & 1)) {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    __atomic_fetch_or(&attr_devs, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
+  }
+  k<<<(unsigned)(g.MT * g.NT * slices), 512, (size_t)G::S * G::KP * G::STG, st>>>(a, g);
 }
 
 template <bool PAIR>
-void launch(GemmI8Args a, void* workspace, hipStream_t st) {
-  // a launch stays within 2^32 threads: 2^22 tiles of 64 x 64
-  const int64_t most = std::max<int64_t>(((int64_t)1 << 22) / (a.N / 64 + 1) * 64 & ~(int64_t)255, 256);
-  for (; a.M > most; a.M -= (int)most) {
-    GemmI8Args part = a;
-    part.M = (int)most;
-    launch<PAIR>(part, workspace, st);
-    const size_t by = (size_t)most * a.N * (a.dtype == VRA_F32 ? 4 : 2);
-    a.x += (size_t)most * a.K, a.xs += most, a.out = static_cast<char*>(a.out) + by;
-    if (a.residual) a.residual = static_cast<const char*>(a.residual) + by;
+void run(const GemmI8Args& a, void* ws, const Choice& c, hipStream_t st) {
+  const bool sixteens = in_sixteens(a);
+  if (c.kind == I8_FEW) {
+    constexpr int one = PAIR ? 2 : 1;
+    if (!sixteens) return few_rows<PAIR, one, true>(a, ws, c.slices, st);
+    if (c.size == 2) return few_rows<PAIR, 2, false>(a, ws, c.slices, st);
+    if (c.size == 4) return few_rows<PAIR, 4, false>(a, ws, c.slices, st);
+    return few_rows<PAIR, PAIR ? 8 : 1, false>(a, ws, c.slices, st);
   }
-  with_type(a.dtype, [&](auto t) {
-    const int cols = (a.N + (PAIR ? 31 : 63)) / (PAIR ? 32 : 64);
-    gemm_i8_any_kernel<decltype(t), PAIR><<<(unsigned)((a.M + 63) / 64 * cols), 256, 0, st>>>(a, cols);
-  });
+  if (c.kind == I8_TILE) {
+    if (c.size == 0x44) return tile<PAIR, 256, 256, false>(a, ws, c.slices, st);
+    if (c.size == 0x34) return tile<PAIR, 192, 256, false>(a, ws, c.slices, st);
+    if (c.size == 0x24) return tile<PAIR, 128, 256, false>(a, ws, c.slices, st);
+    if (c.size == 0x32) return tile<PAIR, 192, 128, false>(a, ws, c.slices, st);
+    if (c.size == 0x22) return tile<PAIR, 128, 128, false>(a, ws, c.slices, st);
+    // 64 x 128: two K steps a phase where every workgroup has a CU to itself, otherwise two workgroups a CU (gemm_rows_launch)
+    if (tile_count(a.M, a.N, PAIR, 0x12) * c.slices <= 256) return tile<PAIR, 64, 128, true>(a, ws, c.slices, st);
+    return tile<PAIR, 64, 128, false>(a, ws, c.slices, st);
+  }
+  const int cols = (int)over(a.N, PAIR ? 32 : 64);
+  const unsigned grid = (unsigned)(over(a.M, 64) * cols);
+  if (a.dtype == VRA_BF16) gemm_i8_any_kernel<BF16, PAIR><<<grid, 256, 0, st>>>(a, cols);
+  else if (PAIR || a.dtype == VRA_F16) gemm_i8_any_kernel<F16, PAIR><<<grid, 256, 0, st>>>(a, cols);
+  else gemm_i8_any_kernel<PlainF32, PAIR><<<grid, 256, 0, st>>>(a, cols);
 }
 
-bool product_ok(const char* who, const GemmI8Args& a, const void* workspace, int tensors) {
-  if (a.M < 0 || a.K <= 0 || a.K > 131071 || a.N <= 0) {
-    vra_set_error("%s: m >= 0, 1 <= k <= 131071 (sums of 32 bits), n >= 1 (m=%d k=%d n=%d)", who, a.M, a.K, a.N);
+void launch(GemmI8Args a, bool pair, void* ws, hipStream_t st) {
+  // a launch stays within 2^32 threads: 2^22 tiles of 64 x 64
+  const int64_t most = std::max<int64_t>((((int64_t)1 << 22) / (a.N / 64 + 1) * 64) & ~(int64_t)255, 256);
+  const bool sixteens = in_sixteens(a);
+  while (a.M > 0) {
+    GemmI8Args part = a;
+    part.M = (int)std::min<int64_t>(a.M, most);
+    const Choice c = choose(pair, part.M, a.N, a.K, ws != nullptr, sixteens);
+    if (pair) run<true>(part, ws, c, st);
+    else run<false>(part, ws, c, st);
+    const size_t by = (size_t)part.M * a.N * (a.dtype == VRA_F32 ? 4 : 2);
+    a.x += (size_t)part.M * a.K, a.xs += part.M, a.out = static_cast<char*>(a.out) + by, a.M -= part.M;
+    if (a.residual) a.residual = static_cast<const char*>(a.residual) + by;
+  }
+}
+
+bool product_ok(const char* who, const GemmI8Args& a, bool pair, const void* workspace) {
+  if (a.M < 0 || a.K <= 0 || a.K > 131071 || a.N <= 0 || a.N > 1 << 24) {
+    vra_set_error("%s: m >= 0, 1 <= k <= 131071 (sums of 32 bits), 1 <= n <= 2^24 (m=%d k=%d n=%d)", who, a.M, a.K, a.N);
     return false;
   }
   const bool f32 = a.dtype == VRA_F32;
-  if (a.dtype != VRA_BF16 && a.dtype != VRA_F16 && !(f32 && tensors == 1)) {
-    vra_set_error("%s: dtype must be bf16/f16%s", who, tensors == 1 ? "/f32" : "");
+  if (a.dtype != VRA_BF16 && a.dtype != VRA_F16 && !(f32 && !pair)) {
+    vra_set_error("%s: dtype must be bf16/f16%s", who, pair ? "" : "/f32");
     return false;
   }
   if (a.M == 0) return true;
-  bool null = !a.x || !a.xs || !a.out;
-  uintptr_t words = (uintptr_t)a.xs;
-  for (int t = 0; t < tensors; t++) null |= !a.w[t] || !a.ws[t], words |= (uintptr_t)a.ws[t];
-  if (null) {
+  if (!a.x || !a.xs || !a.out || !a.w[0] || !a.ws[0] || (pair && (!a.w[1] || !a.ws[1]))) {
     vra_set_error("%s: null pointer", who);
     return false;
   }
-  if (words % 4 || ((uintptr_t)a.bias | (uintptr_t)a.residual | (uintptr_t)a.out) % (f32 ? 4 : 2)) {
+  if (((uintptr_t)a.xs | (uintptr_t)a.ws[0] | (uintptr_t)a.ws[1]) % 4 || ((uintptr_t)a.bias | (uintptr_t)a.residual | (uintptr_t)a.out) % (f32 ? 4 : 2)) {
     vra_set_error("%s: a pointer that is not a multiple of its elements' size", who);
     return false;
   }
@@ -61,15 +181,39 @@ bool product_ok(const char* who, const GemmI8Args& a, const void* workspace, int
 
 }  // namespace
 
-extern "C" size_t vra_w8a8_workspace_bytes(void) { return 16; }
+extern "C" size_t vra_w8a8_workspace_bytes(void) { return I8_WS_BYTES; }
 
 extern "C" void vra_w8a8_gemm(const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales, const void* bias, const void* residual, void* out,
                               void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream) {
   const GemmI8Args a = {x, x_scales, {w, nullptr}, {w_scales, nullptr}, bias, residual, out, m, n, k, dtype};
-  if (product_ok("vra_w8a8_gemm", a, workspace, 1) && m) launch<false>(a, workspace, as_stream(stream));
+  if (product_ok("vra_w8a8_gemm", a, false, workspace)) launch(a, false, workspace, as_stream(stream));
 }
 extern "C" void vra_w8a8_gate_up_silu(const int8_t* x, const float* x_scales, const int8_t* w_gate, const float* s_gate, const int8_t* w_up, const float* s_up,
                                       void* out, void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream) {
   const GemmI8Args a = {x, x_scales, {w_gate, w_up}, {s_gate, s_up}, nullptr, nullptr, out, m, n, k, dtype};
-  if (product_ok("vra_w8a8_gate_up_silu", a, workspace, 2) && m) launch<true>(a, workspace, as_stream(stream));
+  if (product_ok("vra_w8a8_gate_up_silu", a, true, workspace)) launch(a, true, workspace, as_stream(stream));
+}
+
+extern "C" int32_t vra_w8a8_kernel(int32_t pair, int32_t m, int32_t k, int32_t n, int32_t has_workspace) {
+  if (m <= 0 || k <= 0 || k > 131071 || n <= 0 || n > 1 << 24) return 0;
+  const Choice c = choose(pair != 0, m, n, k, has_workspace != 0, k % 16 == 0);
+  return c.slices << 16 | c.kind << 8 | c.size;
+}
+extern "C" void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales, const int8_t* w_up, const float* s_up,
+                                 const void* bias, const void* residual, void* out, void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream) {
+  const bool pair = w_up != nullptr;
+  const GemmI8Args a = {x, x_scales, {w, w_up}, {w_scales, s_up}, bias, residual, out, m, n, k, dtype};
+  if (!product_ok("vra_w8a8_gemm_on", a, pair, workspace) || m == 0) return;
+  const Choice c = {kernel >> 8 & 255, kernel & 255, kernel >> 16};
+  bool has = !(pair && (bias || residual)) && (int64_t)m * n <= (int64_t)1 << 34 && c.slices >= 1 && (c.slices == 1 || workspace);
+  if (c.kind == I8_FEW) {
+    has = has && few_has(pair, m, c.size) && slices_fit(c.slices, k, few_tiles(n, pair, c.size), few_bytes(pair, m, c.size)) && (in_sixteens(a) || (c.size == (pair ? 2 : 1) && c.slices == 1));
+  } else if (c.kind == I8_TILE) {
+    has = has && tile_has(c.size) && in_sixteens(a) && (c.size <= 0x32 ? slices_fit(c.slices, k, tile_count(m, n, pair, c.size), (c.size >> 4) * (c.size & 15) * 16384) : c.slices == 1);
+  } else {
+    has = has && c.kind == I8_ANY && c.size == 0 && c.slices == 1;
+  }
+  VRA_CHECK_ARG(has, "vra_w8a8_gemm_on: no such kernel for this product");
+  if (pair) run<true>(a, workspace, c, as_stream(stream));
+  else run<false>(a, workspace, c, as_stream(stream));
 }
