@@ -238,18 +238,20 @@ def test_gate_up_silu(dt, M, work):
         check_product(r, M, K, N, dt, pair=True, work=work)
 
 
-KERNELS = [(1, c, s) for c in (1, 2, 4, 8) for s in (1, 2, 8)] + [(2, t, s) for t in (0x12, 0x22, 0x32, 0x24) for s in (1, 2, 4, 8)] + [(2, 0x34, 1), (2, 0x44, 1)]
+KERNELS = [(1, c, s) for c in (1, 2, 4, 8) for s in (1, 2, 8)] + [(2, t, s) for t in (0x12, 0x22, 0x32, 0x24) for s in (1, 2, 4, 8)] + [(2, 0x34, 1), (2, 0x44, 1)] + [(0, t, s) for t in (0x11, 0x22) for s in (1, 2, 4, 8)]
 
 
 @pytest.mark.parametrize("pair", [False, True])
 @pytest.mark.parametrize("kind, size, slices", KERNELS)
 def test_named_kernels(kind, size, slices, pair, work):
-    """every kernel at the edges of its tiles, in K steps of 128 (one, an odd number, a part behind them, 16 of the last), against the kernel for any alignment: the same bits"""
+    """every kernel at the edges of its tiles, in K steps of 128 (one, an odd number, a part behind them, 16 of the last), against 64-row tiles of the kernel for any alignment:
+    the same bits; that one, and its own, against the definition"""
     L, r = ops.lib(), rng(size * 8 + slices)
     blocks = 16 if kind == 1 else size // 16 * 64
-    rows = {1: [1, 15, 16, 17, 33, 48, 64], 2: [1, blocks - 1, blocks, blocks + 1, 2 * blocks + 3]}[kind]
+    rows = [1, 15, 16, 17, 33, 48, 64] if kind == 1 else [1, blocks - 1, blocks, blocks + 1, 2 * blocks + 3]
     for i, M in enumerate(rows):
         for j, (K, N) in enumerate([(1024, 300), (1168, 257), (1408, 64), (2032, 516), (3216, 8)] if kind == 1 or slices > 1 else [(128, 300), (16, 257), (384, 64), (496, 516), (656, 8)]):
+            K += 3 * (kind == 0 and j < 4)
             dt = [BF16, F16, BF16 if pair else F32][(i + j) % 3]
             x, xs = some_codes(r, M, K)
             w, ws = some_codes(r, N, K)
@@ -258,11 +260,11 @@ def test_named_kernels(kind, size, slices, pair, work):
             d = [ops.dev(t) for t in (x, xs, w, ws, w2, ws2, bias, res)]
             kind_np, size_np = (np.float32, 4) if dt == F32 else (np.uint16, 2)
             got = []
-            for code in (0x10000, slices << 16 | kind << 8 | size):
+            for code in (0x10011, slices << 16 | kind << 8 | size):
                 out = Guarded(M * N * size_np)
                 L.vra_w8a8_gemm_on(code, *[t.ptr for t in d[:4]], *([t.ptr for t in d[4:6]] if pair else [None, None]), None if pair or j % 2 else d[6].ptr,
                                    None if pair or i % 2 else d[7].ptr, out.at, work.ptr, M, K, N, dt, 0)
-                if code != 0x10000 and L.vra_last_error().decode():
+                if code != 0x10011 and L.vra_last_error().decode():
                     assert "no such kernel" in L.vra_last_error().decode()
                     mt = (M + 15) // 16  # only what the table of kernels lacks: few rows beyond a size's blocks
                     assert kind == 1 and (mt > (4 if size <= 2 else 2 if size == 4 else 1) or (size == 1) == pair and size in (1, 8) or size == 8 and not pair)
@@ -272,10 +274,9 @@ def test_named_kernels(kind, size, slices, pair, work):
                 ops.check_error()
                 got.append(out.take(kind_np, (M, N)))
             assert np.array_equal(got[0], got[1]), f"{M} x {N}, K = {K}"
-            if i == 1 and j == 1:
-                ref, bound = plain.gate_up_silu(x, xs, w, ws, w2, ws2, dt) if pair else plain.gemm(x, xs, w, ws, None, None, dt)
-                if pair or M % 2:
-                    plain.assert_within(plain.wide(got[0], dt), ref, bound, "any alignment")
+            if kind == 0 or i == j == 1:
+                ref, bound = plain.gate_up_silu(x, xs, w, ws, w2, ws2, dt) if pair else plain.gemm(x, xs, w, ws, None if j % 2 else bias, None if i % 2 else res, dt)
+                plain.assert_within(plain.wide(got[0], dt), ref, bound, f"any alignment, {M} x {N}, K = {K}")
 
 
 @pytest.mark.parametrize("M, K, N", [(1, 512, 96), (8, 1024, 64), (40, 256, 200), (150, 640, 300), (300, 384, 520)])

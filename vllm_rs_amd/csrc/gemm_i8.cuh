@@ -37,50 +37,7 @@ struct GemmI8Args {
   int dtype;    // of out, bias and residual
 };
 
-// four consecutive columns n .. n + 3 (those within N) of row m
-template <class T>
-__device__ __forceinline__ void load4(float (&f)[4], const void* p, size_t at, int n, int N, bool whole) {
-  const uint16_t* const h = static_cast<const uint16_t*>(p) + at;
-  if (whole) {
-    const u32x2 v = *reinterpret_cast<const u32x2*>(h);
-#pragma unroll
-    for (int e = 0; e < 4; e++) f[e] = T::to_f32((uint16_t)(v[e >> 1] >> (e & 1 ? 16 : 0)));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; e++) f[e] = n + e < N ? T::to_f32(h[e]) : 0.f;
-  }
-}
-struct PlainF32 {};  // (VRA_F32 as a type of the epilogue)
-template <>
-__device__ __forceinline__ void load4<PlainF32>(float (&f)[4], const void* p, size_t at, int n, int N, bool whole) {
-  const float* const h = static_cast<const float*>(p) + at;
-  if (whole) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(h);
-#pragma unroll
-    for (int e = 0; e < 4; e++) f[e] = v[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; e++) f[e] = n + e < N ? h[e] : 0.f;
-  }
-}
-template <class T>
-__device__ __forceinline__ void store4(const float (&f)[4], void* p, size_t at, int n, int N, bool whole) {
-  uint16_t* const h = static_cast<uint16_t*>(p) + at;
-  if (whole) *reinterpret_cast<u32x2*>(h) = u32x2{T::pack2(f[0], f[1]), T::pack2(f[2], f[3])};
-  else
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (n + e < N) h[e] = T::from_f32(f[e]);
-}
-template <>
-__device__ __forceinline__ void store4<PlainF32>(const float (&f)[4], void* p, size_t at, int n, int N, bool whole) {
-  float* const h = static_cast<float*>(p) + at;
-  if (whole) *reinterpret_cast<f32x4*>(h) = f32x4{f[0], f[1], f[2], f[3]};
-  else
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (n + e < N) h[e] = f[e];
-}
+struct PlainF32 {};  // VRA_F32 as a type of the epilogue
 
 // an element as it is stored, and its value
 __device__ __forceinline__ uint32_t load1(int dtype, const void* p, size_t at) {
@@ -92,12 +49,6 @@ __device__ __forceinline__ float value1(int dtype, uint32_t v) {
 __device__ __forceinline__ void store1(int dtype, float v, void* p, size_t at) {
   if (dtype == VRA_F32) static_cast<float*>(p)[at] = v;
   else static_cast<uint16_t*>(p)[at] = dtype == VRA_BF16 ? BF16::from_f32(v) : F16::from_f32(v);
-}
-
-// whether four columns at a multiple of 4 may be read and written at once, in all rows
-__host__ __device__ __forceinline__ bool i8_whole_fours(const GemmI8Args& a) {
-  const uintptr_t all = (uintptr_t)a.out | (uintptr_t)a.residual | (uintptr_t)a.bias;
-  return a.N % 4 == 0 && all % (a.dtype == VRA_F32 ? 16 : 8) == 0;
 }
 
 // what stands behind the sums g (and u) of an element
@@ -113,67 +64,52 @@ __device__ __forceinline__ float i8_value(int g, int u, float xs, float gs, floa
   asm("" : "+v"(v));  // (the last product is not drawn into a conversion to f16, here or there: the bits are the same in all kernels)
   return v;
 }
-// what the epilogue reads of four columns n .. n + 3: the same for all rows
-struct I8Columns {
-  float g[4], u[4], bias[4];
-};
-template <class T, bool PAIR>
-__device__ __forceinline__ I8Columns i8_columns(const GemmI8Args& a, int n, bool whole) {
-  I8Columns c = {};
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int at = min(n + e, a.N - 1);
-    c.g[e] = a.ws[0][at];
-    if (PAIR) c.u[e] = a.ws[1][at];
-  }
-  if (!PAIR && a.bias && n < a.N) load4<T>(c.bias, a.bias, n, n, a.N, whole && n + 4 <= a.N);
-  return c;
-}
-// sums g (and u) of columns n .. n + 3 of row m
-template <class T, bool PAIR>
-__device__ __forceinline__ void i8_store(const GemmI8Args& a, const I8Columns& c, float xs, int m, int n, bool whole, i32x4 g, i32x4 u) {
-  if (m >= a.M || n >= a.N) return;
-  whole = whole && n + 4 <= a.N;
-  const size_t at = (size_t)m * a.N + n;
-  float y[4], f[4];
-#pragma unroll
-  for (int e = 0; e < 4; e++) y[e] = i8_value<PAIR>(g[e], u[e], xs, c.g[e], c.u[e]);
-  if (!PAIR) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) y[e] += c.bias[e];
-    if (a.residual) {
-      load4<T>(f, a.residual, at, n, a.N, whole);
-#pragma unroll
-      for (int e = 0; e < 4; e++) y[e] += f[e];
-    }
-  }
-  store4<T>(y, a.out, at, n, a.N, whole);
-}
-
-// whether eight columns at a multiple of 8 (f32: four at a multiple of 4) are 16 bytes on their place, in all rows
-__host__ __device__ __forceinline__ bool i8_sixteens(const GemmI8Args& a) {
-  return a.N % (a.dtype == VRA_F32 ? 4 : 8) == 0 && ((uintptr_t)a.out | (uintptr_t)a.residual | (uintptr_t)a.bias) % 16 == 0;
-}
+// rows begin anywhere: 16 bytes at a multiple of an element
 typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
-// A wave's R blocks of 16 rows x 64 virtual columns (acc[block][tile of 16 columns]) for i8_sixteens: lane (r16, q4) holds columns 4 q4 .. + 3 of the tiles, of row r16 of the
-// blocks.  m: that row in block 0; n0: the wave's first column.  What is read of rows and columns is asked for together, the residual two blocks ahead (one
-// after the other, they were 30 of a 256 x 256 tile's 39 us behind its loop); 16-bit results trade places between a row's four lanes and go out 16 bytes a lane.
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+// A wave's R blocks of 16 rows x 64 virtual columns: lane (r16, q4) holds columns 4 q4 .. + 3 of the four tiles of a block (acc[block][tile]), of its row r16.  m: that row in
+// block 0; n0: the wave's first column.  What is read of rows and columns is asked for together, the residual two blocks ahead (one after the other, they were 30
+// of a 256 x 256 tile's 39 us behind its loop); 16-bit results trade places between a row's four lanes and go out 16 bytes a lane.
 template <class T, bool PAIR, int R>
 __device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0, int q4, const i32x4 (&acc)[R][4]) {
   constexpr int NJ = PAIR ? 2 : 4;
   constexpr bool F32 = std::is_same<T, PlainF32>::value;
   typedef typename std::conditional<F32, f32x4, u32x2>::type Four;
+  typedef typename std::conditional<F32, f32x4_a4, u32x2_a2>::type FourAnywhere;
+  typedef typename std::conditional<F32, float, uint16_t>::type One;
   const int M = a.M, N = a.N;
   float gs[NJ][4], us[NJ][4], xs[R];
   Four bias[NJ], res[2][NJ];
-  auto fetch = [&](int i) {
-    const size_t row = (size_t)min(m + i * 16, M - 1) * N;
+  // columns n .. n + 3 of a row at p, those within N
+  auto four = [&](const void* p, int n, Four& v) {
+    const One* const h = static_cast<const One*>(p) + n;
+    if (n + 4 <= N) v = *reinterpret_cast<const FourAnywhere*>(h);
+    else if (n < N) {
+      v = Four{};
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const size_t at = row + min(n0 + j * 16 + q4 * 4, N - 4);
-      if constexpr (F32) res[i & 1][j] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.residual) + at);
-      else res[i & 1][j] = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.residual) + at);
+      for (int e = 0; e < 3; e++)
+        if (n + e < N) {
+          if constexpr (F32) v[e] = h[e];
+          else v[e >> 1] |= (uint32_t)h[e] << (e & 1 ? 16 : 0);
+        }
     }
+  };
+  auto scales = [&](const float* p, int n, float (&f)[4]) {
+    if (n + 4 <= N) {
+      const f32x4 v = *reinterpret_cast<const f32x4_a4*>(p + n);
+#pragma unroll
+      for (int e = 0; e < 4; e++) f[e] = v[e];
+    } else if (n < N) {
+#pragma unroll
+      for (int e = 0; e < 3; e++)
+        if (n + e < N) f[e] = p[n + e];
+    }
+  };
+  auto fetch = [&](int i) {
+    const One* const row = static_cast<const One*>(a.residual) + (size_t)min(m + i * 16, M - 1) * N;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) four(row, n0 + j * 16 + q4 * 4, res[i & 1][j]);
   };
   const bool has_res = !PAIR && a.residual, has_bias = !PAIR && a.bias;
   if (has_res) {
@@ -182,14 +118,10 @@ __device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0
   }
 #pragma unroll
   for (int j = 0; j < NJ; j++) {
-    const int n = min(n0 + j * 16 + q4 * 4, N - 4);
-    const f32x4 g = *reinterpret_cast<const f32x4_a4*>(a.ws[0] + n), u = PAIR ? (f32x4)*reinterpret_cast<const f32x4_a4*>(a.ws[1] + n) : g;
-#pragma unroll
-    for (int e = 0; e < 4; e++) gs[j][e] = g[e], us[j][e] = u[e];
-    if (has_bias) {
-      if constexpr (F32) bias[j] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.bias) + n);
-      else bias[j] = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.bias) + n);
-    }
+    const int n = n0 + j * 16 + q4 * 4;
+    scales(a.ws[0], n, gs[j]);
+    if (PAIR) scales(a.ws[1], n, us[j]);
+    if (has_bias) four(a.bias, n, bias[j]);
   }
 #pragma unroll
   for (int i = 0; i < R; i++) xs[i] = a.xs[min(m + i * 16, M - 1)];
@@ -206,18 +138,22 @@ __device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[j][e] = i8_value<PAIR>(acc[i][PAIR ? 2 * j : j][e], acc[i][PAIR ? 2 * j + 1 : j][e], xs[i], gs[j][e], us[j][e]);
+      for (int e = 0; e < 4; e++) y[j][e] = i8_value<PAIR>(acc[i][PAIR ? 2 * j : j][e], acc[i][PAIR ? 2 * j + 1 : j][e], xs[i], gs[j][e], PAIR ? us[j][e] : 0.f);
       if (has_bias) add(y[j], bias[j]);
       if (has_res) add(y[j], res[i & 1][j]);
     }
     if (has_res && i + 2 < R) fetch(i + 2);
     const bool in = m + i * 16 < M;
-    const size_t row = (size_t)(m + i * 16) * N;
+    One* const row = static_cast<One*>(a.out) + (size_t)(m + i * 16) * N;
     if constexpr (F32) {
 #pragma unroll
       for (int j = 0; j < NJ; j++) {
         const int n = n0 + j * 16 + q4 * 4;
-        if (in && n < N) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + row + n) = f32x4{y[j][0], y[j][1], y[j][2], y[j][3]};
+        if (in && n + 4 <= N) *reinterpret_cast<f32x4_a4*>(row + n) = f32x4{y[j][0], y[j][1], y[j][2], y[j][3]};
+        else if (in)
+#pragma unroll
+          for (int e = 0; e < 3; e++)
+            if (n + e < N) row[n + e] = y[j][e];
       }
     } else {
       u32x2 v[NJ];
@@ -227,75 +163,47 @@ __device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0
 #pragma unroll
       for (int h = 0; h < NJ / 2; h++) {
         const int n = n0 + q4 * (NJ * 4) + h * 8;
-        if (in && n < N) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + row + n) = u32x4{v[2 * h][0], v[2 * h][1], v[2 * h + 1][0], v[2 * h + 1][1]};
+        const u32x4 p = {v[2 * h][0], v[2 * h][1], v[2 * h + 1][0], v[2 * h + 1][1]};
+        if (in && n + 8 <= N) *reinterpret_cast<u32x4_a2*>(row + n) = p;
+        else if (in)
+#pragma unroll
+          for (int e = 0; e < 7; e++)
+            if (n + e < N) row[n + e] = (uint16_t)(p[e >> 1] >> (e & 1 ? 16 : 0));
       }
     }
   }
 }
+template <bool PAIR, int R>
+__device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0, int q4, const i32x4 (&acc)[R][4]) {
+  if (a.dtype == VRA_BF16) i8_store_rows<BF16, PAIR, R>(a, m, n0, q4, acc);
+  else if (PAIR || a.dtype == VRA_F16) i8_store_rows<F16, PAIR, R>(a, m, n0, q4, acc);
+  else if constexpr (!PAIR) i8_store_rows<PlainF32, PAIR, R>(a, m, n0, q4, acc);
+}
 
-// ---------------------------------------------------------------- any K, any alignment
-// 64 rows x 64 columns (pair: 32 gate and 32 up columns, interleaved in blocks of 16) a workgroup of four waves, 32 x 32 each; steps of 64 k through two
-// buffers of LDS, filled through registers by loads of 16 bytes at any address (bytes one by one where K ends inside them).
-template <class T, bool PAIR>
-__global__ __launch_bounds__(256) void gemm_i8_any_kernel(const GemmI8Args a, int cols) {
-#ifdef __HIP_DEVICE_COMPILE__
-  constexpr int P = 80;  // bytes from row to row in LDS
-  __shared__ __attribute__((aligned(16))) unsigned char buf[2][2][64 * P];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
-  const int K = a.K, mt = (int)blockIdx.x / cols, m0 = mt * 64, n0 = ((int)blockIdx.x - mt * cols) * (PAIR ? 32 : 64);
-  const int row = tid >> 2, chunk = (tid & 3) * 16;
-  // (virtual column `row` of a pair: block row / 16, of tensor block & 1)
-  const int col = min(n0 + (PAIR ? (row >> 5) * 16 + (row & 15) : row), a.N - 1);
-  const int8_t* const xp = a.x + (size_t)min(m0 + row, a.M - 1) * K;
-  const int8_t* const wp = (PAIR && (row & 16) ? a.w[1] : a.w[0]) + (size_t)col * K;
-  auto load16 = [&](const int8_t* p, int k) {
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (k + 16 <= K) return *reinterpret_cast<const u32x4_a1*>(p + k);
+// 16 bytes of a row of K from byte k on (k a multiple of 16), zeros behind the row's end; any address, nothing beyond the row is read
+__device__ __forceinline__ u32x4 i8_load16(const int8_t* row, int k, int K) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (k + 16 <= K) return *reinterpret_cast<const u32x4_a1*>(row + k);
+  if (k < K) {
+    const int left = K - k;
+    if (K >= 16) {  // the row's last 16 bytes, the first of them shifted out
+      const u32x4 t = *reinterpret_cast<const u32x4_a1*>(row + K - 16);
+      const int d = (16 - left) >> 2, b = (16 - left) & 3;
+      uint32_t s[8];
 #pragma unroll
-    for (int e = 0; e < 15; e++)
-      if (k + e < K) v[e >> 2] |= (uint32_t)(uint8_t)p[k + e] << (8 * (e & 3));
-    return (u32x4_a1)v;
-  };
-  auto put = [&](int b, u32x4 x, u32x4 w) {
-    *reinterpret_cast<u32x4*>(&buf[b][0][row * P + chunk]) = x;
-    *reinterpret_cast<u32x4*>(&buf[b][1][row * P + chunk]) = w;
-  };
-  i32x4 acc[2][2];
+      for (int i = 0; i < 8; i++) s[i] = i < 4 ? t[i] : 0u;
 #pragma unroll
-  for (int i = 0; i < 4; i++) acc[i >> 1][i & 1] = zero_acc_i8();
-  const int xr = (wave >> 1) * 32, wr = (wave & 1) * 32;
-  put(0, load16(xp, chunk), load16(wp, chunk));
-  __syncthreads();
-  for (int k = 0, b = 0; k < K; k += 64, b ^= 1) {
-    u32x4 nx = {}, nw = {};
-    const bool more = k + 64 < K;
-    if (more) nx = load16(xp, k + 64 + chunk), nw = load16(wp, k + 64 + chunk);
-    u32x4 xf[2], wf[2];
+      for (int i = 0; i < 4; i++) {
+        const uint32_t lo = d == 0 ? s[i] : d == 1 ? s[i + 1] : d == 2 ? s[i + 2] : s[i + 3], hi = d == 0 ? s[i + 1] : d == 1 ? s[i + 2] : d == 2 ? s[i + 3] : s[i + 4];
+        v[i] = __builtin_amdgcn_alignbyte(hi, lo, b);
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      xf[i] = *reinterpret_cast<const u32x4*>(&buf[b][0][(xr + i * 16 + r16) * P + q4 * 16]);
-      wf[i] = *reinterpret_cast<const u32x4*>(&buf[b][1][(wr + i * 16 + r16) * P + q4 * 16]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < 2; j++) mfma_i8(acc[i][j], wf[j], xf[i]);
-    if (more) put(b ^ 1, nx, nw);
-    __syncthreads();
-  }
-  VRA_MFMA_DRAIN();
-  const bool whole = i8_whole_fours(a);
-#pragma unroll
-  for (int j = 0; j < (PAIR ? 1 : 2); j++) {
-    const int n = n0 + (PAIR ? wr >> 1 : wr + j * 16) + q4 * 4;
-    const I8Columns c = i8_columns<T, PAIR>(a, n, whole);
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int m = m0 + xr + i * 16 + r16;
-      i8_store<T, PAIR>(a, c, a.xs[min(m, a.M - 1)], m, n, whole, acc[i][j], acc[i][1]);
+      for (int e = 0; e < 15; e++)
+        if (e < left) v[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
     }
   }
-#endif
+  return v;
 }
 
 // ---------------------------------------------------------------- few rows (decode)
@@ -425,20 +333,11 @@ __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Arg
   if ((K & 127) && z == slices - 1 && wave == whole % NW) {  // what K leaves behind whole steps; a chunk beyond it counts nothing, as its x is zero
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const int k = whole * 128 + q4 * 32 + h * 16, at = whole * 128 + h * 16, left = K - k;
-      auto take = [&](const int8_t* p) {
-        u32x4 v = {0u, 0u, 0u, 0u};
-        if (left >= 16) v = ANY ? (u32x4)*reinterpret_cast<const u32x4_a1*>(p + at) : *reinterpret_cast<const u32x4*>(p + at);
-        else if (ANY)
+      const int k = whole * 128 + q4 * 32 + h * 16;
 #pragma unroll
-          for (int e = 0; e < 15; e++)
-            if (e < left) v[e >> 2] |= (uint32_t)(uint8_t)p[at + e] << (8 * (e & 3));
-        return v;
-      };
+      for (int c = 0; c < C; c++) w[0][c][h] = i8_load16(wp[c] - q4 * 32, k, K);
 #pragma unroll
-      for (int c = 0; c < C; c++) w[0][c][h] = take(wp[c]);
-#pragma unroll
-      for (int i = 0; i < MT; i++) x[0][i][h] = take(xp[i]);
+      for (int i = 0; i < MT; i++) x[0][i][h] = i8_load16(xp[i] - q4 * 32, k, K);
     }
     product(0);
   }
@@ -679,23 +578,105 @@ __global__ __launch_bounds__(512, 2) void gemm_i8_tile_kernel(const GemmI8Args a
       for (int i = 0; i < NX * 16; i++) acc[i >> 4][i >> 2 & 3][i & 3] = v[i];
     }
   }
-  const bool sixteens = i8_sixteens(a), whole = i8_whole_fours(a);
-  auto finish = [&](auto t) {
-    using T = decltype(t);
-    if (sixteens) return i8_store_rows<T, PAIR, H * NX>(a, m0 + row0 + r16, n0 + (PAIR ? cw * 32 : cw * 64), q4, acc);
+  i8_store_rows<PAIR, H * NX>(a, m0 + row0 + r16, n0 + (PAIR ? cw * 32 : cw * 64), q4, acc);
+#endif
+}
+
+// ---------------------------------------------------------------- many rows, any K, any alignment
+// Rows that begin anywhere cannot go to LDS by themselves: they come through registers, 16 bytes at any address a load, two K steps of 128 ahead of the one in
+// LDS (one step of 64 ahead: 777 x 1003, K = 2741 31 us, nearly all of it waiting).  Four waves: BN = 64: 16 rows each, BN = 128: 64 x 64 each.  PAIR: virtual columns,
+// gate and up interleaved in blocks of 16.  LDS as above, two buffers.
+template <bool PAIR, int BM, int BN>
+__global__ __launch_bounds__(256, 2) void gemm_i8_any_kernel(const GemmI8Args a, const GemmI8Tiles g) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int CW = BN / 64, R = BM * CW / 64, XE = BM / 32, WE = BN / 32, STG = (BM + BN) * 128;  // blocks of 16 rows of a wave; 16-byte pieces of a thread
+  __shared__ __attribute__((aligned(16))) unsigned char buf[2 * STG];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), cw = wave % CW, rw = wave / CW;
+  const int tiles = g.MT * g.NT, z = (int)blockIdx.x % g.slices, lin = (int)blockIdx.x / g.slices;
+  int mt, nt;
+  gr_tile_of(lin, g.MT, g.NT, mt, nt);
+  const int K = a.K, KT = (K + 127) >> 7, ks0 = (int)((int64_t)KT * z / g.slices), ks1 = (int)((int64_t)KT * (z + 1) / g.slices);
+  const int m0 = mt * BM, n0 = nt * (PAIR ? BN / 2 : BN);
+  // piece e of a thread: 16-byte chunk tid & 7 of row (tid >> 3) + 32 e
+  const int ch = tid & 7, r8 = tid >> 3;
+  const int8_t* xp[XE];
+  const int8_t* wp[WE];
 #pragma unroll
-    for (int j = 0; j < (PAIR ? 2 : 4); j++) {
-      const int n = n0 + (PAIR ? cw * 32 : cw * 64) + j * 16 + q4 * 4;
-      const I8Columns c = i8_columns<T, PAIR>(a, n, whole);
+  for (int e = 0; e < XE; e++) xp[e] = a.x + (size_t)min(m0 + r8 + 32 * e, a.M - 1) * K;
 #pragma unroll
-      for (int i = 0; i < H * NX; i++) {
-        const int m = m0 + row0 + i * 16 + r16;
-        i8_store<T, PAIR>(a, c, a.xs[min(m, a.M - 1)], m, n, whole, acc[i][PAIR ? 2 * j : j], acc[i][PAIR ? 2 * j + 1 : j]);
-      }
+  for (int e = 0; e < WE; e++) {
+    const int v = r8 + 32 * e, row = PAIR ? (v >> 5) * 16 + (v & 15) : v;
+    wp[e] = (PAIR && (v & 16) ? a.w[1] : a.w[0]) + (size_t)min(n0 + row, a.N - 1) * K;
+  }
+  const int slot = r8 * 128 + ((ch ^ (r8 & 7)) * 16);
+  u32x4 xr[2][XE], wr[2][WE];
+  auto load = [&](int b, int ks) __attribute__((always_inline)) {
+    if (ks >= ks1) return;
+    const int k = ks * 128 + ch * 16;
+    if (ks * 128 + 128 <= K) {
+#pragma unroll
+      for (int e = 0; e < XE; e++) xr[b][e] = *reinterpret_cast<const u32x4_a1*>(xp[e] + k);
+#pragma unroll
+      for (int e = 0; e < WE; e++) wr[b][e] = *reinterpret_cast<const u32x4_a1*>(wp[e] + k);
+    } else {
+#pragma unroll
+      for (int e = 0; e < XE; e++) xr[b][e] = i8_load16(xp[e], k, K);
+#pragma unroll
+      for (int e = 0; e < WE; e++) wr[b][e] = i8_load16(wp[e], k, K);
     }
   };
-  if (a.dtype == VRA_BF16) finish(BF16{});
-  else if (PAIR || a.dtype == VRA_F16) finish(F16{});
-  else finish(PlainF32{});
+  auto put = [&](int b, int o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < XE; e++) *reinterpret_cast<u32x4*>(buf + o + slot + e * 4096) = xr[b][e];
+#pragma unroll
+    for (int e = 0; e < WE; e++) *reinterpret_cast<u32x4*>(buf + o + BM * 128 + slot + e * 4096) = wr[b][e];
+  };
+  const int c0 = r16 * 128 + (q4 ^ (r16 & 7)) * 16;
+  i32x4 acc[R][4];
+#pragma unroll
+  for (int i = 0; i < R; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = zero_acc_i8();
+  // K step ks is in buffer b; register set b (steps of the same parity) holds step ks + 2 on its way, the other one step ks + 1
+  auto step = [&](auto B, int ks) __attribute__((always_inline)) {
+    constexpr int b = decltype(B)::value, o = b * STG;
+    if (ks < ks1) {
+#pragma unroll
+      for (int kc = 0; kc < 2; kc++) {
+        u32x4 xa[R], wa[4];
+#pragma unroll
+        for (int i = 0; i < R; i++) xa[i] = *reinterpret_cast<const u32x4*>(buf + o + (c0 ^ (kc * 64)) + (rw * R + i) * 2048);
+#pragma unroll
+        for (int j = 0; j < 4; j++) wa[j] = *reinterpret_cast<const u32x4*>(buf + o + BM * 128 + (c0 ^ (kc * 64)) + (cw * 4 + j) * 2048);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) mfma_i8(acc[i][j], wa[j], xa[i]);
+      }
+    }
+    if (ks + 1 < ks1) put(1 - b, STG - o);
+    load(1 - b, ks + 3);
+    __syncthreads();
+  };
+  load(0, ks0);
+  load(1, ks0 + 1);
+  put(0, 0);
+  load(0, ks0 + 2);
+  __syncthreads();
+  for (int ks = ks0; ks < ks1; ks += 2) {
+    step(std::integral_constant<int, 0>{}, ks);
+    step(std::integral_constant<int, 1>{}, ks + 1);
+  }
+  VRA_MFMA_DRAIN();
+  if (g.slices > 1) {
+    int v[R * 16];
+#pragma unroll
+    for (int i = 0; i < R * 16; i++) v[i] = acc[i >> 4][i >> 2 & 3][i & 3];
+    if (!i8_meet<R * 16, 256>(v, g.ws, lin, tiles, z, g.slices, reinterpret_cast<int*>(buf))) return;
+#pragma unroll
+    for (int i = 0; i < R * 16; i++) acc[i >> 4][i >> 2 & 3][i & 3] = v[i];
+  }
+  i8_store_rows<PAIR, R>(a, m0 + rw * R * 16 + r16, n0 + (PAIR ? cw * 32 : cw * 64), q4, acc);
 #endif
 }
