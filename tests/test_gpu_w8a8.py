@@ -81,8 +81,8 @@ def some_rows(r, rows, cols, dt):
     return plain.to(x, dt)
 
 
-# widths at the edges of a vector, of a wave's, 256 threads' and 1024 threads' registers, and past them
-WIDTHS = [1, 2, 7, 8, 9, 63, 64, 513, 1001, 2047, 2048, 2049, 2056, 4096, 5632, 8191, 8192, 8193, 18944, 32768, 32769, 32776, 131072]
+# widths at the edges of a vector, of what 64 .. 1024 threads keep in registers, and past it
+WIDTHS = [1, 2, 7, 8, 9, 63, 64, 512, 513, 519, 520, 1001, 1024, 1032, 2047, 2048, 2056, 4096, 4103, 4104, 5632, 8191, 8192, 8193, 8200, 14336, 16391, 16392, 18944, 24576, 24584, 32768, 32776, 131072]
 
 
 @pytest.mark.parametrize("kind", ["quant", "norm", "add"])
@@ -102,6 +102,15 @@ def test_rows_that_begin_anywhere(kind, rows, cols, shift):
     r = rng(rows + cols)
     x, res, w = some_rows(r, rows, cols, BF16), some_rows(r, rows, cols, BF16), plain.to(1 + 0.2 * r.standard_normal(cols), BF16)
     check_rows(kind, x, BF16, rows_of(kind, x, BF16, res, w, shift), res, w)
+
+
+@pytest.mark.parametrize("kind", ["quant", "norm", "add"])
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("cols", [1024, 1031, 1032, 4096, 4104, 8192, 8203, 16384, 16400, 24576])
+def test_many_rows(kind, dt, cols):
+    r = rng(cols + dt)
+    x, res, w = some_rows(r, 513, cols, dt), some_rows(r, 513, cols, dt), plain.to(1 + 0.2 * r.standard_normal(cols), dt)
+    check_rows(kind, x, dt, rows_of(kind, x, dt, res, w), res, w)
 
 
 @pytest.mark.parametrize("in_place", ["x", "residual"])

@@ -5,7 +5,8 @@
 //
 // The norm's factor is the same for a whole row: it is in the scale, and not in q.  Products of two 16-bit floats are exact in f32, and a quotient within the
 // f32 division's error of a half is decided by its exact remainder: q is the definition's, bit for bit, whatever the order of the sums.
-// Bound: memory.  A row is read once and kept in registers as it came (the sum as it is stored) between the reduction and the quotients.
+// Bound: memory, and close behind it the vector instructions, 12 an element without a norm and 18 with one (8192 x 4096 bf16: sum and norm 41.0 us = 5.7 TB/s, norm 23.5, neither 23.5 = 4.3;
+// 3063 x 18944 f16 37.1 = 4.7).  A row is read once and kept in registers as it came (the sum as it is stored) between the reduction and the quotients.
 #include <type_traits>
 
 #include "common.cuh"
@@ -69,9 +70,11 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_i8_kernel(const RowsI8
   const bool has_tail = n && tid == T - 1;  // the elements behind the last eight
   const size_t at = (size_t)row * cols;
   u32x4 keep[V ? V : 1], wk[V ? V : 1], keep_t, wk_t;
-  double sum = 0.0;  // (squares of bf16 leave f32's range at 2^64; an f64 multiply-add runs at the f32 rate)
+  double sum = 0.0;  // (squares of bf16 leave f32's range at 2^64)
   uint32_t top = 0u;  // |p| as bits: ordered as the values are, infinities and NaN above all others
-  auto first = [&](auto tail, int c, u32x4& kept, u32x4& wv) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 top2 = {0, 0};  // the same of the elements as they are stored (no norm), two at a time
+  auto first = [&](auto tail, int c, u32x4& kept, u32x4& wv) __attribute__((always_inline)) {
     constexpr bool TL = decltype(tail)::value;
     u32x4 v = load8<TL>(a.x + at + c, n);
     float f[8];
@@ -90,15 +93,18 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_i8_kernel(const RowsI8
           if (e < n) a.h_out[at + c + e] = (uint16_t)(v[e >> 1] >> (e & 1 ? 16 : 0));
     }
     kept = v;
-    unpack8<DT>(v, f);
     if (NORM) {
       float w[8];
+      unpack8<DT>(v, f);
       unpack8<DT>(wv, w);
 #pragma unroll
       for (int e = 0; e < 8; e++) sum = fma((double)f[e], (double)f[e], sum), f[e] *= w[e];
-    }
 #pragma unroll
-    for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+      for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+    }
   };
   if constexpr (V > 0) {
 #pragma unroll
@@ -108,6 +114,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_i8_kernel(const RowsI8
     for (int c = tid * 8; c < whole; c += T * 8) first(std::false_type{}, c, keep[0], wk[0]);
   }
   if (has_tail) first(std::true_type{}, whole, keep_t, wk_t);
+  if (!NORM) top = __float_as_uint(DT::to_f32(max(top2[0], top2[1])));
   row_reduce<T, NORM>(sum, top);
   // a row that is not finite in 32 bits: codes 0 and scale NaN, which makes NaN of all that is computed from it
   const bool finite = top < 0x7f800000u && sum < (double)INFINITY;  // (an infinity or NaN times a weight of zero is in the sum)
@@ -116,12 +123,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_i8_kernel(const RowsI8
     const double s = (double)amax / 127.0;
     a.scales[row] = finite ? (float)(NORM ? s / sqrt(sum / cols + (double)a.eps) : s) : __uint_as_float(0x7fc00000u);
   }
-  // the range's ends are moved to its middle, by a power of two: neither 127 / a nor 127 p overflows, no remainder is lost below the normal range
-  const float shift = amax < 0x1p-60f ? 0x1p64f : amax > 0x1p60f ? 0x1p-64f : 1.0f;
-  const float as = amax * shift, inv = finite && top ? 127.0f / as : 0.f;
-  auto second = [&](auto tail, int c, const u32x4& v, const u32x4& wv) {
+  // the lower end of the range is moved up by a power of two: 127 / a does not overflow, no remainder is lost below the normal range
+  const bool tiny = __builtin_amdgcn_readfirstlane(amax < 0x1p-60f);
+  const float as = tiny ? amax * 0x1p64f : amax, inv = top ? 127.0f / as : 0.f;
+  auto second = [&](auto tail, int c, u32x4 v, u32x4 wv) __attribute__((always_inline)) {
     constexpr bool TL = decltype(tail)::value;
-    float f[8], r[8];
+    constexpr float WHOLE = 12582912.0f;  // 1.5 2^23: a sum with it is a whole number, rounded to even, whose lowest byte is the 8-bit integer
+    float f[8], r[8], far = 0.f;
     unpack8<DT>(v, f);
     if (NORM) {
       float w[8];
@@ -129,27 +137,33 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_i8_kernel(const RowsI8
 #pragma unroll
       for (int e = 0; e < 8; e++) f[e] *= w[e];
     }
-    bool close = false;
+    if (tiny)
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] *= 0x1p64f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      f[e] = finite ? f[e] * shift : 0.f;
       const float t = f[e] * inv;  // |t| <= 127 (1 + 2^-22): off by less than 2^-15
-      r[e] = rintf(t);
-      close |= fabsf(t - r[e]) > 0.5f - 0x1p-14f;
+      r[e] = t + WHOLE;
+      far = fmaxf(far, fabsf(t - (r[e] - WHOLE)));
     }
-    if (close) {
+    if (far > 0.5f - 0x1p-14f) {
       // 127 p = hi + lo exactly; d = hi - r a is exact: |d| is about a / 2, a multiple of both units and within 24 bits of the larger one.  2 |d + lo| against a
-      // says on which side of the half the quotient lies
+      // says on which side of the half the quotient lies.  (127 p of the range's upper end: both moved down)
+      const float down = as > 0x1p60f ? 0x1p-64f : 1.0f, ad = as * down;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float hi = 127.0f * f[e], lo = fmaf(127.0f, f[e], -hi), d = fmaf(-r[e], as, hi);
-        const float up = d > 0.f ? 1.f : -1.f, over = fmaf(2.0f, fabsf(d), -as) + 2.0f * up * lo;
-        if (over > 0.f || (over == 0.f && ((int)r[e] & 1))) r[e] += up;
+        const float p = f[e] * down, q = r[e] - WHOLE, hi = 127.0f * p, lo = fmaf(127.0f, p, -hi), d = fmaf(-q, ad, hi);
+        const float up = d > 0.f ? 1.f : -1.f, over = fmaf(2.0f, fabsf(d), -ad) + 2.0f * up * lo;
+        if (over > 0.f || (over == 0.f && ((int)q & 1))) r[e] += up;
       }
     }
-    u32x2 o = {0u, 0u};
+    u32x2 o;
 #pragma unroll
-    for (int e = 0; e < 8; e++) o[e >> 2] |= ((uint32_t)(int)r[e] & 0xffu) << (8 * (e & 3));
+    for (int h = 0; h < 2; h++) {
+      const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(r[4 * h + 1]), __float_as_uint(r[4 * h]), 0x0c0c0400u);
+      const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(r[4 * h + 3]), __float_as_uint(r[4 * h + 2]), 0x0c0c0400u);
+      o[h] = finite ? lo | hi << 16 : 0u;
+    }
     int8_t* const to = a.q + at + c;
     if (!TL) *reinterpret_cast<u32x2_a1*>(to) = o;
     else
@@ -181,10 +195,28 @@ void launch(RowsI8Args a, hipStream_t st) {
     a.x += by, a.q += by, a.scales += most;
     if (MODE == QI_ADD_NORM) a.residual += by, a.h_out += by;
   }
-  if (a.cols <= 2048) rows_i8_kernel<DT, MODE, 64, 4><<<(a.rows + 3) / 4, 256, 0, st>>>(a);
-  else if (a.cols <= 8192) rows_i8_kernel<DT, MODE, 256, 4><<<a.rows, 256, 0, st>>>(a);
-  else if (a.cols <= 32768) rows_i8_kernel<DT, MODE, 1024, 4><<<a.rows, 1024, 0, st>>>(a);
-  else rows_i8_kernel<DT, MODE, 1024, 0><<<a.rows, 1024, 0, st>>>(a);
+  // Threads of a row and the eights each keeps.  Few rows (two workgroups a CU at most): as many threads as there are eights, the row is one round trip (16 x 14336: 256 threads 9.2 us,
+  // 512 5.7, 1024 4.5).  Many: two eights and more a thread, so that the barrier and the reduction stand behind more requests (8192 x 4096: 512 threads 27.9 us, 256 23.5; 8192 x 1024: 256 threads
+  // 11.8, one wave 9.6), beyond 8192 as many as keep their registers (4096 x 14336, no norm: 1024 threads 43.5 us, 512 39.6; norm and sum: 75.3 / 78.1)
+  const int whole = a.cols & ~7;
+  const bool many = a.rows > 512;
+  auto go = [&](auto t, auto v) {
+    constexpr int T = decltype(t)::value, V = decltype(v)::value;
+    rows_i8_kernel<DT, MODE, T, V><<<T == 64 ? (a.rows + 3) / 4 : a.rows, T == 64 ? 256 : T, 0, st>>>(a);
+  };
+#define QI_KERNEL(T, V) go(std::integral_constant<int, T>{}, std::integral_constant<int, V>{})
+  if (whole <= (many ? 1024 : 512)) QI_KERNEL(64, 2);
+  else if (!many && whole <= 2048) QI_KERNEL(256, 1);
+  else if (!many && whole <= 4096) QI_KERNEL(512, 1);
+  else if (!many && whole <= 8192) QI_KERNEL(1024, 1);
+  else if (whole <= 4096) QI_KERNEL(256, 2);
+  else if (whole <= 8192) QI_KERNEL(512, 2);
+  else if (many && MODE == QI_PLAIN && whole <= 16384) QI_KERNEL(512, MODE == QI_PLAIN ? 4 : 2);
+  else if (whole <= 16384) QI_KERNEL(1024, 2);
+  else if (whole <= 24576) QI_KERNEL(1024, 3);
+  else if (whole <= 32768) QI_KERNEL(1024, 4);
+  else QI_KERNEL(1024, 0);
+#undef QI_KERNEL
 }
 
 template <int MODE>
