@@ -207,20 +207,21 @@ __device__ __forceinline__ u32x4 i8_load16(const int8_t* row, int k, int K) {
 }
 
 // ---------------------------------------------------------------- few rows (decode)
-// Where the K slices of a product meet: a partial tile of every slice but the last to arrive, and a counter a tile (a line each), zero between calls.
-#define I8_WS_COUNTERS 1024
-#define I8_WS_PARTIALS ((size_t)I8_WS_COUNTERS * 64)
+// Where the K slices of a product meet: the sums of every slice, and a counter for each wave of a tile (a line each), zero between calls.
+#define I8_WS_TILES 1024
+#define I8_WS_PARTIALS ((size_t)I8_WS_TILES * 8 * 64)
 #define I8_WS_PARTIAL_BYTES ((size_t)32 << 20)
 #define I8_WS_BYTES (I8_WS_PARTIALS + I8_WS_PARTIAL_BYTES)
 
-// Stores `n` sums a thread (v) of slice `z` of a tile and returns whether this workgroup is the tile's last: then the other slices' sums have been added to v, and the counter
-// is zero again.  All threads call it; `flag`: a word of LDS that nobody reads or writes by other means any more.  Nobody waits for anybody.  Sums go through memory with agent scope (sc1: the L2s of the XCDs are not
-// coherent), each store is acknowledged before its workgroup counts itself, and the last one reads behind all counts.
+// A wave stores its V sums a lane of slice z and counts itself; the last of the `slices` waves of the same place of the tile adds the others' sums to its own, sets the counter back and
+// returns true.  Nobody waits for anybody, and where slices end together their waves share the work.  Sums go through memory with agent scope (sc1: the L2s of the XCDs are
+// not coherent); a wave's stores are acknowledged before it counts itself, and the last one reads behind all counts.  It asks for several slices at a time: one after the other they were
+// 0.8 .. 1.7 us each, and a workgroup's waves waited for its last (150 x 3584, K = 18944, four slices of 128 x 128: 31.4 us, so 26.8; 32 x 512, K = 14336, eight slices: 8.9, 7.6).
 template <int V, int THREADS>
-__device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int tiles, int z, int slices, int* flag) {
+__device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int tiles, int z, int slices) {
+  constexpr int W = V % 4 ? 1 : 4, B = V <= 16 ? 4 : V <= 32 ? 3 : 2;  // sums a load; slices in flight
   const int tid = threadIdx.x;
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(static_cast<char*>(ws) + I8_WS_PARTIALS, 0, 0x7FFFFFF0, 0x00020000u);
-  constexpr int W = V % 4 ? 1 : 4;  // sums a store
   auto at = [&](int s, int i) { return (uint32_t)(((s * tiles + tile) * (V / W) + i) * THREADS + tid) * (4u * W); };
 #pragma unroll
   for (int i = 0; i < V / W; i++) {
@@ -228,35 +229,36 @@ __device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int til
     else __builtin_amdgcn_raw_buffer_store_b32((uint32_t)v[i], r, at(z, i), 0, 16);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  uint32_t* const count = static_cast<uint32_t*>(ws) + tile * 16;
-  if (tid == 0) *flag = (int)__hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == slices - 1;
-  __syncthreads();
-  if (!*flag) return false;
-  for (int s = 0; s < slices; s++) {
-    if (s == z) continue;
-    if constexpr (W == 4) {
-      u32x4 p[V / 4];
+  uint32_t* const count = static_cast<uint32_t*>(ws) + (tile * 8 + (tid >> 6)) * 16;
+  uint32_t before = 0u;
+  if ((tid & 63) == 0) before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  before = __builtin_amdgcn_readfirstlane(before);
+  asm volatile("" ::: "memory");
+  if (before != (uint32_t)slices - 1u) return false;
+  for (int s0 = 1; s0 < slices; s0 += B) {
+    u32x4 p[B][(V + 3) / 4];
 #pragma unroll
-      for (int i = 0; i < V / 4; i++) p[i] = __builtin_amdgcn_raw_buffer_load_b128(r, at(s, i), 0, 16);
+    for (int b = 0; b < B; b++) {
+      const int s = z + s0 + b, o = s0 + b < slices ? (s >= slices ? s - slices : s) : z;  // (behind the last: its own again, not added)
 #pragma unroll
-      for (int i = 0; i < V; i++) v[i] += (int)p[i >> 2][i & 3];
-    } else {
-      uint32_t p[V];
-#pragma unroll
-      for (int i = 0; i < V; i++) p[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at(s, i), 0, 16);
-#pragma unroll
-      for (int i = 0; i < V; i++) v[i] += (int)p[i];
+      for (int i = 0; i < V / W; i++) {
+        if constexpr (W == 4) p[b][i] = __builtin_amdgcn_raw_buffer_load_b128(r, at(o, i), 0, 16);
+        else p[b][i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b32(r, at(o, i), 0, 16);
+      }
     }
+#pragma unroll
+    for (int b = 0; b < B; b++)
+      if (s0 + b < slices)
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] += (int)p[b][i >> 2][i & 3];
   }
-  if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if ((tid & 63) == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return true;
 }
 
 #define I8_NW 8
 // Bound: the weights' way through memory.  A workgroup takes 16 C virtual columns (pair: gate and up blocks of 16 in turn), all MT 16 rows and one of `slices` runs of
-// K; its eight waves take the run's steps of 128 in turn, straight into registers, U of them asked for at once (a lane: 32 bytes of its row, so that a wave's request covers whole
-// lines).  The waves' sums meet in LDS, the slices' in the workspace.  ANY: rows that begin anywhere, or K off 16.
+// K; its eight waves take the run's steps of 128 in turn, straight into registers, U of them asked for at once.  The waves' sums meet in LDS, the slices' in the workspace.  ANY: rows that begin anywhere, or K off 16.
 template <bool PAIR, int MT, int C, int U, bool ANY>
 __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Args a, void* ws, int slices) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -266,17 +268,19 @@ __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Arg
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int M = a.M, N = a.N, K = a.K, tile = (int)blockIdx.x / slices, z = (int)blockIdx.x - tile * slices, n0 = tile * CO * 16;
+  // a lane's two pieces of a step: one of each half, so that a request is for 64 bytes of a row.  It meets fewer lines than one for 128 where rows do not begin with one (pieces side by side / so:
+  // pair 11 x 9216, K = 9264 50.0 / 46.8 us, 11 x 17024, K = 4384 26.8 / 24.1; whole lines 1 % slower, and with the form by K 7 %, for its registers)
   const int8_t* wp[C];
   const int8_t* xp[MT];
 #pragma unroll
-  for (int c = 0; c < C; c++) wp[c] = (PAIR && (c & 1) ? a.w[1] : a.w[0]) + (size_t)min(n0 + (PAIR ? c >> 1 : c) * 16 + r16, N - 1) * K + q4 * 32;
+  for (int c = 0; c < C; c++) wp[c] = (PAIR && (c & 1) ? a.w[1] : a.w[0]) + (size_t)min(n0 + (PAIR ? c >> 1 : c) * 16 + r16, N - 1) * K + q4 * 16;
 #pragma unroll
-  for (int i = 0; i < MT; i++) xp[i] = a.x + (size_t)min(i * 16 + r16, M - 1) * K + q4 * 32;
+  for (int i = 0; i < MT; i++) xp[i] = a.x + (size_t)min(i * 16 + r16, M - 1) * K + q4 * 16;
   u32x4 w[U][C][2], x[U][MT][2];
   auto load = [&](int u, int step) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const int at = step * 128 + h * 16;
+      const int at = step * 128 + h * 64;
 #pragma unroll
       for (int c = 0; c < C; c++) w[u][c][h] = ANY ? (u32x4)*reinterpret_cast<const u32x4_a1*>(wp[c] + at) : *reinterpret_cast<const u32x4*>(wp[c] + at);
 #pragma unroll
@@ -333,11 +337,11 @@ __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Arg
   if ((K & 127) && z == slices - 1 && wave == whole % NW) {  // what K leaves behind whole steps; a chunk beyond it counts nothing, as its x is zero
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const int k = whole * 128 + q4 * 32 + h * 16;
+      const int k = whole * 128 + h * 64 + q4 * 16;
 #pragma unroll
-      for (int c = 0; c < C; c++) w[0][c][h] = i8_load16(wp[c] - q4 * 32, k, K);
+      for (int c = 0; c < C; c++) w[0][c][h] = i8_load16(wp[c] - q4 * 16, k, K);
 #pragma unroll
-      for (int i = 0; i < MT; i++) x[0][i][h] = i8_load16(xp[i] - q4 * 32, k, K);
+      for (int i = 0; i < MT; i++) x[0][i][h] = i8_load16(xp[i] - q4 * 16, k, K);
     }
     product(0);
   }
@@ -362,7 +366,8 @@ __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Arg
     sums[e] = g;
     if (PAIR) sums[E + e] = u;
   }
-  if (slices > 1 && !i8_meet<E * (PAIR ? 2 : 1), NW * 64>(sums, ws, tile, (int)gridDim.x / slices, z, slices, part)) return;
+  if (slices > 1 && wave * 64 >= OUT) return;  // (a wave without results)
+  if (slices > 1 && !i8_meet<E * (PAIR ? 2 : 1), NW * 64>(sums, ws, tile, (int)gridDim.x / slices, z, slices)) return;
 #pragma unroll
   for (int e = 0; e < E; e++) {
     if (!in[e]) continue;
@@ -570,10 +575,11 @@ __global__ __launch_bounds__(512, 2) void gemm_i8_tile_kernel(const GemmI8Args a
   VRA_MFMA_DRAIN();
   if constexpr (H == 1) {
     if (g.slices > 1) {
+      if (!in) return;
       int v[NX * 16];
 #pragma unroll
       for (int i = 0; i < NX * 16; i++) v[i] = acc[i >> 4][i >> 2 & 3][i & 3];
-      if (!i8_meet<NX * 16, 512>(v, g.ws, lin, tiles, z, g.slices, reinterpret_cast<int*>(smem))) return;
+      if (!i8_meet<NX * 16, 512>(v, g.ws, lin, tiles, z, g.slices)) return;
 #pragma unroll
       for (int i = 0; i < NX * 16; i++) acc[i >> 4][i >> 2 & 3][i & 3] = v[i];
     }
@@ -673,7 +679,7 @@ __global__ __launch_bounds__(256, 2) void gemm_i8_any_kernel(const GemmI8Args a,
     int v[R * 16];
 #pragma unroll
     for (int i = 0; i < R * 16; i++) v[i] = acc[i >> 4][i >> 2 & 3][i & 3];
-    if (!i8_meet<R * 16, 256>(v, g.ws, lin, tiles, z, g.slices, reinterpret_cast<int*>(buf))) return;
+    if (!i8_meet<R * 16, 256>(v, g.ws, lin, tiles, z, g.slices)) return;
 #pragma unroll
     for (int i = 0; i < R * 16; i++) acc[i >> 4][i >> 2 & 3][i & 3] = v[i];
   }

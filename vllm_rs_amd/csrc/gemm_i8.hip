@@ -27,42 +27,44 @@ int64_t tile_bytes(int t) { return (t >> 4) * (t & 15) * 16384; }  // of its sum
 bool tile_has(int t) { return t == 0x12 || t == 0x22 || t == 0x32 || t == 0x24 || t == 0x34 || t == 0x44; }
 // whether `slices` runs of K have a step each and meet within the workspace
 bool slices_fit(int slices, int K, int64_t tiles, int64_t tile_bytes) {
-  return slices == 1 || ((slices == 2 || slices == 4 || slices == 8) && slices <= K / 128 && tiles <= I8_WS_COUNTERS && tiles * slices * tile_bytes <= (int64_t)I8_WS_PARTIAL_BYTES);
+  return slices == 1 || ((slices == 2 || slices == 4 || slices == 8) && slices <= K / 128 && tiles <= I8_WS_TILES && tiles * slices * tile_bytes <= (int64_t)I8_WS_PARTIAL_BYTES);
 }
 int64_t few_bytes(bool pair, int M, int C) {  // of a workgroup's sums, in whole rounds of its threads
   const int CO = pair ? C / 2 : C;
   return over((int64_t)(M + 15) / 16 * CO * 256, I8_NW * 64) * I8_NW * 64 * 4 * (pair ? 2 : 1);
 }
 
-// Times in us, fitted to 2100 (few) and 2400 (tile) measured ones: 1..64 and 17..8192 rows, 15 products of K = 992..18944 and 512..32000 columns, weights from memory, rms 12 and 7..13 %; the
-// choice by them is 1.0 % behind the best one measured on average, 22 % at most (48 rows x 5632 + 5632, K = 2048).
-// few: what the busiest CU reads, at 35 GB/s, and what the chip reads, weights at 6.55 TB/s and the rows of x, once a workgroup, at 13.9; the longer of them and a quarter of the other
+// Times in us, fitted to 916 (few) and 2957 (tile) measured ones: 1..64 and 17..8192 rows, 16 products of K = 992..18944 and 512..32000 columns, weights from memory, rms 13 and 5..10 %; the
+// choice by them is 0.8 % behind the best one measured on average, 25 % at most (48 rows x 5632 + 5632, K = 2048).
+// few: what the busiest CU reads, at 35 GB/s, and what the chip reads, weights at 6.1 TB/s and the rows of x, once a workgroup, at 14.1; the longer of them and a quarter of the other
 double few_us(bool pair, int M, int N, int K, int C, int slices) {
   const double wgs = (double)few_tiles(N, pair, C) * slices, t = pair ? 2 : 1;
   const double cu = (double)over((int64_t)wgs, 256) * (16.0 * C + M) * K / slices / 34.9e3;
-  const double chip = t * N * K / 6.55e6 + wgs / slices * M * K / 13.9e6;
-  return 2.41 + (slices > 1 ? 0.82 + 0.50 * slices : 0.0) + std::max(cu, chip) + 0.245 * std::min(cu, chip);
+  const double chip = t * N * K / 6.06e6 + wgs / slices * M * K / 14.1e6;
+  return 2.69 + (slices > 1 ? 1.48 + 0.235 * slices : 0.0) + std::max(cu, chip) + 0.247 * std::min(cu, chip);
 }
 // tile: as in gemm_rows_tile (gemm_rows.cuh): rounds of 256 workgroups (64 x 128 on few: two a CU), for each a fixed time and one for each K step, the last round's between that of few workgroups
-// and of all; and the slices' meeting.  Never quicker than the weights' way through memory.
+// and of all, less by the share `rows` of it where the last tile row is not full; never quicker than the weights' way through memory; and the slices' meeting, for each of them and for each MB
+// that they write and read
 double tile_us(bool pair, int M, int N, int K, int t, int slices) {
   const int64_t wgs = tile_count(M, N, pair, t) * slices;
   const bool deep = t == 0x12 && wgs <= 256;
-  struct Times { int tile; double t0, round, one, half, full, meet, slice; };
-  static const Times times[7] = {{0x12, 2.7, 4.33, 0.421, 0.679, 0.695, 3.53, 0.99}, {0x22, 0.0, 5.79, 0.429, 0, 0.566, 0.77, 1.28}, {0x32, 2.2, 3.10, 0.560, 0, 0.762, 1.32, 1.65},
-                                 {0x24, 2.9, 2.86, 0.710, 0, 0.987, 2.22, 1.74}, {0x34, 0.6, 6.33, 0.803, 0, 1.121, 0, 0}, {0x44, 0.0, 8.24, 0.930, 0, 1.438, 0, 0},
-                                 {0x12, 0.8, 3.57, 0.363, 0, 0.493, 0.85, 0.79}};
+  struct Times { int tile; double t0, round, one, half, full, rows, meet, slice, mb; };
+  static const Times times[7] = {{0x12, 3.1, 2.72, 0.474, 0.745, 0.693, 0.0, 0.0, 0.87, 0.164}, {0x22, 0.5, 4.25, 0.510, 0, 0.524, 0.466, 0.0, 0.77, 0.203},
+                                 {0x32, 0.7, 4.41, 0.610, 0, 0.689, 0.151, 0.0, 0.97, 0.176}, {0x24, 0.0, 5.58, 0.771, 0, 0.858, 0.32, 0.0, 1.28, 0.155},
+                                 {0x34, 0.7, 6.53, 0.821, 0, 1.080, 0.289, 0, 0, 0}, {0x44, 0.0, 8.78, 0.984, 0, 1.374, 0.517, 0, 0, 0},
+                                 {0x12, 1.6, 2.53, 0.388, 0, 0.433, 0.207, 0.34, 0.53, 0.25}};
   const Times* c = &times[6];
   if (!deep)
     for (c = times; c->tile != t;) c++;
-  const int slots = t == 0x12 && !deep ? 512 : 256;
-  const double full = (double)(wgs / slots), rem = (double)(wgs % slots), steps = (double)over(K, 128) / slices;
+  const int bm = (t >> 4) * 64, bn = (t & 15) * 64, slots = t == 0x12 && !deep ? 512 : 256;
+  const double full = (double)(wgs / slots), rem = (double)(wgs % slots), steps = (double)over(K, 128) / slices, rows = (double)M / over(M, bm);
   double last = rem > 0 ? c->one + (c->full - c->one) * rem / slots : 0.0;
   if (slots == 512 && rem > 0) last = rem <= 256 ? c->one : c->half + (c->full - c->half) * (rem - 256) / 256;
-  const double us = c->t0 + (full + (rem > 0)) * c->round + steps * (full * c->full + last) + (slices > 1 ? c->meet + c->slice * slices : 0.0);
-  return std::max(us, 3.0 + (pair ? 2.0 : 1.0) * N * K / 6.3e6);
+  const double fill = 1.0 - c->rows + c->rows * (bn + rows) / (bn + bm);
+  const double us = std::max(c->t0 + (full + (rem > 0)) * c->round + steps * fill * (full * c->full + last), 3.0 + (pair ? 2.0 : 1.0) * N * K / 6.3e6);
+  return slices == 1 ? us : us + c->meet + c->slice * slices + c->mb * wgs * rows * bn * 8e-6;
 }
-
 // rows that begin anywhere, 850 times of 1..8192 rows, rms 13..15 %, the choice 2.4 % behind the best on average: the same forms.  any: two workgroups a CU, a K step's time a constant
 // and one for each of the CU's workgroups
 double few_any_us(bool pair, int M, int N, int K) {
