@@ -39,18 +39,6 @@ struct GemmI8Args {
 
 struct PlainF32 {};  // VRA_F32 as a type of the epilogue
 
-// an element as it is stored, and its value
-__device__ __forceinline__ uint32_t load1(int dtype, const void* p, size_t at) {
-  return dtype == VRA_F32 ? static_cast<const uint32_t*>(p)[at] : static_cast<const uint16_t*>(p)[at];
-}
-__device__ __forceinline__ float value1(int dtype, uint32_t v) {
-  return dtype == VRA_F32 ? __uint_as_float(v) : dtype == VRA_BF16 ? BF16::to_f32((uint16_t)v) : F16::to_f32((uint16_t)v);
-}
-__device__ __forceinline__ void store1(int dtype, float v, void* p, size_t at) {
-  if (dtype == VRA_F32) static_cast<float*>(p)[at] = v;
-  else static_cast<uint16_t*>(p)[at] = dtype == VRA_BF16 ? BF16::from_f32(v) : F16::from_f32(v);
-}
-
 // what stands behind the sums g (and u) of an element
 template <bool PAIR>
 __device__ __forceinline__ float i8_value(int g, int u, float xs, float gs, float us) {
@@ -68,6 +56,22 @@ __device__ __forceinline__ float i8_value(int g, int u, float xs, float gs, floa
 typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
 typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+// columns n .. n + 3 (those within N) of a row of 16- or 32-bit elements as they are stored; the others are left alone
+template <class One, class V>
+__device__ __forceinline__ void i8_four(const void* row, int n, int N, V& v) {
+  typedef typename std::conditional<sizeof(One) == 4, f32x4_a4, u32x2_a2>::type Anywhere;
+  const One* const h = static_cast<const One*>(row) + n;
+  if (n + 4 <= N) v = *reinterpret_cast<const Anywhere*>(h);
+  else if (n < N) {
+    v = V{};
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+      if (n + e < N) {
+        if constexpr (sizeof(One) == 4) v[e] = h[e];
+        else v[e >> 1] |= (uint32_t)h[e] << (e & 1 ? 16 : 0);
+      }
+  }
+}
 // A wave's R blocks of 16 rows x 64 virtual columns: lane (r16, q4) holds columns 4 q4 .. + 3 of the four tiles of a block (acc[block][tile]), of its row r16.  m: that row in
 // block 0; n0: the wave's first column.  What is read of rows and columns is asked for together, the residual two blocks ahead (one after the other, they were 30
 // of a 256 x 256 tile's 39 us behind its loop); 16-bit results trade places between a row's four lanes and go out 16 bytes a lane.
@@ -76,40 +80,20 @@ __device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0
   constexpr int NJ = PAIR ? 2 : 4;
   constexpr bool F32 = std::is_same<T, PlainF32>::value;
   typedef typename std::conditional<F32, f32x4, u32x2>::type Four;
-  typedef typename std::conditional<F32, f32x4_a4, u32x2_a2>::type FourAnywhere;
   typedef typename std::conditional<F32, float, uint16_t>::type One;
   const int M = a.M, N = a.N;
   float gs[NJ][4], us[NJ][4], xs[R];
   Four bias[NJ], res[2][NJ];
-  // columns n .. n + 3 of a row at p, those within N
-  auto four = [&](const void* p, int n, Four& v) {
-    const One* const h = static_cast<const One*>(p) + n;
-    if (n + 4 <= N) v = *reinterpret_cast<const FourAnywhere*>(h);
-    else if (n < N) {
-      v = Four{};
-#pragma unroll
-      for (int e = 0; e < 3; e++)
-        if (n + e < N) {
-          if constexpr (F32) v[e] = h[e];
-          else v[e >> 1] |= (uint32_t)h[e] << (e & 1 ? 16 : 0);
-        }
-    }
-  };
   auto scales = [&](const float* p, int n, float (&f)[4]) {
-    if (n + 4 <= N) {
-      const f32x4 v = *reinterpret_cast<const f32x4_a4*>(p + n);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    i8_four<float>(p, n, N, v);
 #pragma unroll
-      for (int e = 0; e < 4; e++) f[e] = v[e];
-    } else if (n < N) {
-#pragma unroll
-      for (int e = 0; e < 3; e++)
-        if (n + e < N) f[e] = p[n + e];
-    }
+    for (int e = 0; e < 4; e++) f[e] = v[e];
   };
   auto fetch = [&](int i) {
     const One* const row = static_cast<const One*>(a.residual) + (size_t)min(m + i * 16, M - 1) * N;
 #pragma unroll
-    for (int j = 0; j < NJ; j++) four(row, n0 + j * 16 + q4 * 4, res[i & 1][j]);
+    for (int j = 0; j < NJ; j++) i8_four<One>(row, n0 + j * 16 + q4 * 4, N, res[i & 1][j]);
   };
   const bool has_res = !PAIR && a.residual, has_bias = !PAIR && a.bias;
   if (has_res) {
@@ -121,7 +105,7 @@ __device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0
     const int n = n0 + j * 16 + q4 * 4;
     scales(a.ws[0], n, gs[j]);
     if (PAIR) scales(a.ws[1], n, us[j]);
-    if (has_bias) four(a.bias, n, bias[j]);
+    if (has_bias) i8_four<One>(a.bias, n, N, bias[j]);
   }
 #pragma unroll
   for (int i = 0; i < R; i++) xs[i] = a.xs[min(m + i * 16, M - 1)];
@@ -263,7 +247,8 @@ template <bool PAIR, int MT, int C, int U, bool ANY>
 __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Args a, void* ws, int slices) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int NW = I8_NW;
-  constexpr int CO = PAIR ? C / 2 : C, OUT = MT * CO * 256, E = (OUT + NW * 64 - 1) / (NW * 64);  // results of the workgroup, of a thread
+  constexpr int CO = PAIR ? C / 2 : C, FOURS = MT * CO * 64;  // four results a thread
+  static_assert(FOURS <= NW * 64, "a thread has one four");
   __shared__ __attribute__((aligned(16))) int part[NW * MT * C * 256];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -305,22 +290,24 @@ __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Arg
   for (int u = 0; u < U; u++)
 #pragma unroll
     for (int i = 0; i < MT; i++) x[u][i][0] = x[u][i][1] = u32x4{0u, 0u, 0u, 0u};  // (rows beyond M)
-  // the epilogue's operands: element o of the workgroup is column o % 4 + 4 (o / 64 % 4) of block o / 256 % CO, row o / 4 % 16 of block o / (256 CO)
-  float xs[E], gs[E], us[E];
-  uint32_t bias[E], res[E];
-  size_t at[E];
-  bool in[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int o = tid + e * NW * 64, l = o >> 2 & 63, m = o / (256 * CO) * 16 + (l & 15), n = n0 + (o >> 8) % CO * 16 + (l >> 4) * 4 + (o & 3);
-    in[e] = o < OUT && m < M && n < N;
-    at[e] = (size_t)m * N + n;
-    xs[e] = gs[e] = us[e] = 0.f, bias[e] = res[e] = 0u;
-    if (!in[e]) continue;
-    xs[e] = a.xs[m], gs[e] = a.ws[0][n];
-    if (PAIR) us[e] = a.ws[1][n];
-    if (!PAIR && a.bias) bias[e] = load1(a.dtype, a.bias, n);
-    if (!PAIR && a.residual) res[e] = load1(a.dtype, a.residual, at[e]);
+  // the epilogue's operands: thread t has columns 4 (t / 16 % 4) .. + 3 of block t / 64 % CO, row t % 16 of row block t / (64 CO)
+  const int m = tid / (64 * CO) * 16 + r16, n = n0 + (tid >> 6) % CO * 16 + q4 * 4;
+  const bool mine = tid < FOURS && m < M && n < N, f32 = a.dtype == VRA_F32;
+  const size_t row = (size_t)m * N;
+  float xs = 0.f;
+  f32x4 gs = {}, us = {}, bias4 = {}, res4 = {};
+  u32x2 bias2 = {}, res2 = {};
+  if (mine) {
+    xs = a.xs[m];
+    i8_four<float>(a.ws[0], n, N, gs);
+    if (PAIR) i8_four<float>(a.ws[1], n, N, us);
+    else if (f32) {
+      if (a.bias) i8_four<float>(a.bias, n, N, bias4);
+      if (a.residual) i8_four<float>(static_cast<const float*>(a.residual) + row, n, N, res4);
+    } else {
+      if (a.bias) i8_four<uint16_t>(a.bias, n, N, bias2);
+      if (a.residual) i8_four<uint16_t>(static_cast<const uint16_t*>(a.residual) + row, n, N, res2);
+    }
   }
   // steps of 128 of the run, begun at another place in every workgroup: rows of a power of two bytes lie on the same channels of the memory, and all workgroups would ask for the same
   // of them at a time (pair 1 x 14336, K = 4096, in order / so: 24.9 / 22.0 us; K = 3584: no difference)
@@ -351,30 +338,63 @@ __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Arg
 #pragma unroll
     for (int c = 0; c < C; c++) *reinterpret_cast<i32x4*>(&part[((wave * MT + i) * C + c) * 256 + lane * 4]) = acc[i][c];
   __syncthreads();
-  int sums[E * (PAIR ? 2 : 1)];
+  if (wave * 64 >= FOURS) return;
+  int sums[PAIR ? 8 : 4];
+  const int b = tid >> 6;  // block (row block, column block) of the results; its sums are in blocks of C a row block
+  const int* const p = &part[(PAIR ? b * 2 : b) * 256 + lane * 4];
+  i32x4 g = {0, 0, 0, 0}, u = {0, 0, 0, 0};
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int o = tid + e * NW * 64, b = o >> 8;  // block (i, column block) of the results; its sums are in blocks of C a row block
-    const int* p = &part[(PAIR ? b * 2 : b) * 256 + (o & 255)];
-    int g = 0, u = 0;
-    if (o < OUT)
-#pragma unroll
-      for (int v = 0; v < NW; v++) {
-        g += p[v * MT * C * 256];
-        if (PAIR) u += p[v * MT * C * 256 + 256];
-      }
-    sums[e] = g;
-    if (PAIR) sums[E + e] = u;
+  for (int v = 0; v < NW; v++) {
+    g += *reinterpret_cast<const i32x4*>(p + v * MT * C * 256);
+    if (PAIR) u += *reinterpret_cast<const i32x4*>(p + v * MT * C * 256 + 256);
   }
-  if (slices > 1 && wave * 64 >= OUT) return;  // (a wave without results)
-  if (slices > 1 && !i8_meet<E * (PAIR ? 2 : 1), NW * 64>(sums, ws, tile, (int)gridDim.x / slices, z, slices)) return;
+  if (slices > 1) {
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    if (!in[e]) continue;
-    float y = i8_value<PAIR>(sums[e], PAIR ? sums[E + e] : 0, xs[e], gs[e], us[e]);
-    if (!PAIR) y = y + value1(a.dtype, bias[e]) + value1(a.dtype, res[e]);
-    store1(a.dtype, y, a.out, at[e]);
+    for (int e = 0; e < 4; e++) {
+      sums[e] = g[e];
+      if (PAIR) sums[4 + e] = u[e];
+    }
+    if (!i8_meet<PAIR ? 8 : 4, FOURS>(sums, ws, tile, (int)gridDim.x / slices, z, slices)) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      g[e] = sums[e];
+      if (PAIR) u[e] = sums[4 + e];
+    }
   }
+  if (!mine) return;
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) y[e] = i8_value<PAIR>(g[e], u[e], xs, gs[e], us[e]);
+  if (f32) {
+    float* const to = static_cast<float*>(a.out) + row + n;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (a.bias) y[e] += bias4[e];
+      if (a.residual) y[e] += res4[e];
+    }
+    if (n + 4 <= N) *reinterpret_cast<f32x4_a4*>(to) = f32x4{y[0], y[1], y[2], y[3]};
+    else
+#pragma unroll
+      for (int e = 0; e < 3; e++)
+        if (n + e < N) to[e] = y[e];
+    return;
+  }
+  auto store = [&](auto t) {
+    using T = decltype(t);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (!PAIR && a.bias) y[e] += T::to_f32((uint16_t)(bias2[e >> 1] >> (e & 1 ? 16 : 0)));
+      if (!PAIR && a.residual) y[e] += T::to_f32((uint16_t)(res2[e >> 1] >> (e & 1 ? 16 : 0)));
+    }
+    uint16_t* const to = static_cast<uint16_t*>(a.out) + row + n;
+    if (n + 4 <= N) *reinterpret_cast<u32x2_a2*>(to) = u32x2{T::pack2(y[0], y[1]), T::pack2(y[2], y[3])};
+    else
+#pragma unroll
+      for (int e = 0; e < 3; e++)
+        if (n + e < N) to[e] = T::from_f32(y[e]);
+  };
+  if (a.dtype == VRA_BF16) store(BF16{});
+  else store(F16{});
 #endif
 }
 

@@ -29,23 +29,19 @@ bool tile_has(int t) { return t == 0x12 || t == 0x22 || t == 0x32 || t == 0x24 |
 bool slices_fit(int slices, int K, int64_t tiles, int64_t tile_bytes) {
   return slices == 1 || ((slices == 2 || slices == 4 || slices == 8) && slices <= K / 128 && tiles <= I8_WS_TILES && tiles * slices * tile_bytes <= (int64_t)I8_WS_PARTIAL_BYTES);
 }
-int64_t few_bytes(bool pair, int M, int C) {  // of a workgroup's sums, in whole rounds of its threads
-  const int CO = pair ? C / 2 : C;
-  return over((int64_t)(M + 15) / 16 * CO * 256, I8_NW * 64) * I8_NW * 64 * 4 * (pair ? 2 : 1);
-}
+int64_t few_bytes(bool pair, int M, int C) { return (int64_t)((M + 15) / 16) * C * 1024; }  // of a workgroup's sums
 
-// Times in us, fitted to 916 (few) and 2957 (tile) measured ones: 1..64 and 17..8192 rows, 16 products of K = 992..18944 and 512..32000 columns, weights from memory, rms 13 and 5..10 %; the
-// choice by them is 0.8 % behind the best one measured on average, 25 % at most (48 rows x 5632 + 5632, K = 2048).
-// few: what the busiest CU reads, at 35 GB/s, and what the chip reads, weights at 6.1 TB/s and the rows of x, once a workgroup, at 14.1; the longer of them and a quarter of the other
+// Times in us, fitted to 2018 (few) and 2957 (tile) measured ones: 1..64 and 17..8192 rows, 27 products of K = 992..18944 and 192..32000 columns, weights from memory, rms 8 and 5..10 %; the
+// choice by them is 0.7 % (few) and 0.8 % (both) behind the best one measured on average, 17 and 25 % at most.  Rows that are no whole lines of 128 bytes cost more on every way.
+// few: what the busiest CU reads, at 36 GB/s, and the weights at 7.0 TB/s, the longer of them and a quarter of the other; the slices' meeting, for each of them and for each MB that they write and read
 double few_us(bool pair, int M, int N, int K, int C, int slices) {
   const double wgs = (double)few_tiles(N, pair, C) * slices, t = pair ? 2 : 1;
-  const double cu = (double)over((int64_t)wgs, 256) * (16.0 * C + M) * K / slices / 34.9e3;
-  const double chip = t * N * K / 6.06e6 + wgs / slices * M * K / 14.1e6;
-  return 2.69 + (slices > 1 ? 1.48 + 0.235 * slices : 0.0) + std::max(cu, chip) + 0.247 * std::min(cu, chip);
+  const double cu = (double)over((int64_t)wgs, 256) * (16.0 * C + M) * K / slices / 35.9e3 * (K % 128 ? 1.14 : 1.0);
+  const double chip = t * N * K / 7.03e6 * (K % 128 ? 1.53 : 1.0);
+  return 2.73 + (slices > 1 ? 0.92 + slices * (0.175 + 0.596 * over(M, 16) * 16 * N * t * 8e-6) : 0.0) + std::max(cu, chip) + 0.235 * std::min(cu, chip);
 }
 // tile: as in gemm_rows_tile (gemm_rows.cuh): rounds of 256 workgroups (64 x 128 on few: two a CU), for each a fixed time and one for each K step, the last round's between that of few workgroups
-// and of all, less by the share `rows` of it where the last tile row is not full; never quicker than the weights' way through memory; and the slices' meeting, for each of them and for each MB
-// that they write and read
+// and of all, less by the share `rows` of it where the last tile row is not full; never quicker than the weights' way through memory; and the slices' meeting
 double tile_us(bool pair, int M, int N, int K, int t, int slices) {
   const int64_t wgs = tile_count(M, N, pair, t) * slices;
   const bool deep = t == 0x12 && wgs <= 256;
@@ -61,7 +57,7 @@ double tile_us(bool pair, int M, int N, int K, int t, int slices) {
   const double full = (double)(wgs / slots), rem = (double)(wgs % slots), steps = (double)over(K, 128) / slices, rows = (double)M / over(M, bm);
   double last = rem > 0 ? c->one + (c->full - c->one) * rem / slots : 0.0;
   if (slots == 512 && rem > 0) last = rem <= 256 ? c->one : c->half + (c->full - c->half) * (rem - 256) / 256;
-  const double fill = 1.0 - c->rows + c->rows * (bn + rows) / (bn + bm);
+  const double fill = (1.0 - c->rows + c->rows * (bn + rows) / (bn + bm)) * (K % 128 ? 1.35 : 1.0);
   const double us = std::max(c->t0 + (full + (rem > 0)) * c->round + steps * fill * (full * c->full + last), 3.0 + (pair ? 2.0 : 1.0) * N * K / 6.3e6);
   return slices == 1 ? us : us + c->meet + c->slice * slices + c->mb * wgs * rows * bn * 8e-6;
 }
