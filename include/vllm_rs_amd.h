@@ -189,8 +189,8 @@ void vra_w8a8_gemm(const int8_t* x, const float* x_scales, const int8_t* w, cons
 /* the gate / up pair of a feed-forward block (mlp.rs:451-469): out[m, n] = round(silu(g) u), g and u two such products in f32; dtype bf16/f16 */
 void vra_w8a8_gate_up_silu(const int8_t* x, const float* x_scales, const int8_t* w_gate, const float* s_gate, const int8_t* w_up, const float* s_up,
                            void* out, void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype, int64_t stream);
-/* the kernel that they take for a product (its rows, and those of w, on multiples of 16 bytes where k is one), as slices of K << 16 | kind << 8 | size: kind 0 any alignment,
- * 1 few rows (size: 16-column blocks of a workgroup, gate and up counted), 2 tiles (size: rows / 64 * 16 + columns / 64); 0: a shape they refuse */
+/* the kernel that they take for a product (its rows, and those of w, on multiples of 16 bytes where k is one), as slices of K << 16 | kind << 8 | size: kind 1 few rows
+ * (size: 16-column blocks of a workgroup, gate and up counted), 2 tiles and 0 tiles for any alignment (size: rows / 64 * 16 + columns / 64); 0: a shape they refuse */
 int32_t vra_w8a8_kernel(int32_t pair, int32_t m, int32_t k, int32_t n, int32_t has_workspace);
 /* the same products (w_up null: a single one) on a named kernel; the kernel changes no bit of the result */
 void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales, const int8_t* w_up, const float* s_up,

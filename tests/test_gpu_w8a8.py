@@ -247,7 +247,7 @@ def test_gate_up_silu(dt, M, work):
         check_product(r, M, K, N, dt, pair=True, work=work)
 
 
-KERNELS = [(1, c, s) for c in (1, 2, 4, 8) for s in (1, 2, 8)] + [(2, t, s) for t in (0x12, 0x22, 0x32, 0x24) for s in (1, 2, 4, 8)] + [(2, 0x34, 1), (2, 0x44, 1)] + [(0, t, s) for t in (0x11, 0x22) for s in (1, 2, 4, 8)]
+KERNELS = [(1, c, s) for c in (1, 2, 4, 8) for s in (1, 2, 8)] + [(2, t, s) for t in (0x12, 0x22, 0x32, 0x24) for s in (1, 2, 4, 8)] + [(2, 0x34, 1), (2, 0x44, 1)] + [(0, t, s) for t in (0x11, 0x22) for s in (1, 2, 4, 8)] + [(0, 0x44, 1)]
 
 
 @pytest.mark.parametrize("pair", [False, True])

@@ -609,14 +609,16 @@ __global__ __launch_bounds__(512, 2) void gemm_i8_tile_kernel(const GemmI8Args a
 }
 
 // ---------------------------------------------------------------- many rows, any K, any alignment
-// Rows that begin anywhere cannot go to LDS by themselves: they come through registers, 16 bytes at any address a load, two K steps of 128 ahead of the one in
-// LDS (one step of 64 ahead: 777 x 1003, K = 2741 31 us, nearly all of it waiting).  Four waves: BN = 64: 16 rows each, BN = 128: 64 x 64 each.  PAIR: virtual columns,
-// gate and up interleaved in blocks of 16.  LDS as above, two buffers.
-template <bool PAIR, int BM, int BN>
-__global__ __launch_bounds__(256, 2) void gemm_i8_any_kernel(const GemmI8Args a, const GemmI8Tiles g) {
+// Rows that begin anywhere cannot go to LDS by themselves: they come through registers, 16 bytes at any address a load, D K steps of 128 ahead of the one in
+// LDS (one step of 64 ahead: 777 x 1003, K = 2741 31 us, nearly all of it waiting; so 17).  Bound: those loads, which take two turns of a CU's 64 bytes a clock where they are
+// off 16 bytes, beside LDS (8192 x 6144, K = 4097: 128 x 128 362 us, 256 x 256 248: half the loads a product, one step ahead for want of registers).  A wave has 64 virtual columns and R blocks of 16 rows; LDS as above, two
+// buffers.  PAIR: virtual columns, gate and up interleaved in blocks of 16.
+template <bool PAIR, int BM, int BN, int NT, int D>
+__global__ __launch_bounds__(NT, 2) void gemm_i8_any_kernel(const GemmI8Args a, const GemmI8Tiles g) {
 #ifdef __HIP_DEVICE_COMPILE__
-  constexpr int CW = BN / 64, R = BM * CW / 64, XE = BM / 32, WE = BN / 32, STG = (BM + BN) * 128;  // blocks of 16 rows of a wave; 16-byte pieces of a thread
-  __shared__ __attribute__((aligned(16))) unsigned char buf[2 * STG];
+  constexpr int CW = BN / 64, RW = NT / 64 / CW, R = BM / RW / 16, RL = NT / 8, XE = BM / RL, WE = BN / RL, STG = (BM + BN) * 128;  // RL rows a round of loads
+  static_assert(RL % 32 == 0 && R * RW * 16 == BM && XE * RL == BM && WE * RL == BN, "whole rounds");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), cw = wave % CW, rw = wave / CW;
   const int tiles = g.MT * g.NT, z = (int)blockIdx.x % g.slices, lin = (int)blockIdx.x / g.slices;
@@ -624,39 +626,40 @@ __global__ __launch_bounds__(256, 2) void gemm_i8_any_kernel(const GemmI8Args a,
   gr_tile_of(lin, g.MT, g.NT, mt, nt);
   const int K = a.K, KT = (K + 127) >> 7, ks0 = (int)((int64_t)KT * z / g.slices), ks1 = (int)((int64_t)KT * (z + 1) / g.slices);
   const int m0 = mt * BM, n0 = nt * (PAIR ? BN / 2 : BN);
-  // piece e of a thread: 16-byte chunk tid & 7 of row (tid >> 3) + 32 e
+  // piece e of a thread: 16-byte chunk tid & 7 of row (tid >> 3) + RL e
   const int ch = tid & 7, r8 = tid >> 3;
-  const int8_t* xp[XE];
-  const int8_t* wp[WE];
+  const int8_t* const x = a.x + (size_t)m0 * K;
+  const int8_t* const w = (PAIR && (r8 & 16) ? a.w[1] : a.w[0]) + (size_t)n0 * K;
+  uint32_t xo[XE], wo[WE];
 #pragma unroll
-  for (int e = 0; e < XE; e++) xp[e] = a.x + (size_t)min(m0 + r8 + 32 * e, a.M - 1) * K;
+  for (int e = 0; e < XE; e++) xo[e] = (uint32_t)min(r8 + RL * e, a.M - 1 - m0) * (uint32_t)K;
 #pragma unroll
   for (int e = 0; e < WE; e++) {
-    const int v = r8 + 32 * e, row = PAIR ? (v >> 5) * 16 + (v & 15) : v;
-    wp[e] = (PAIR && (v & 16) ? a.w[1] : a.w[0]) + (size_t)min(n0 + row, a.N - 1) * K;
+    const int v = r8 + RL * e;
+    wo[e] = (uint32_t)min(PAIR ? (v >> 5) * 16 + (v & 15) : v, a.N - 1 - n0) * (uint32_t)K;
   }
   const int slot = r8 * 128 + ((ch ^ (r8 & 7)) * 16);
-  u32x4 xr[2][XE], wr[2][WE];
+  u32x4 xr[D][XE], wr[D][WE];
   auto load = [&](int b, int ks) __attribute__((always_inline)) {
     if (ks >= ks1) return;
-    const int k = ks * 128 + ch * 16;
+    const uint32_t k = (uint32_t)ks * 128u + ch * 16u;
     if (ks * 128 + 128 <= K) {
 #pragma unroll
-      for (int e = 0; e < XE; e++) xr[b][e] = *reinterpret_cast<const u32x4_a1*>(xp[e] + k);
+      for (int e = 0; e < XE; e++) xr[b][e] = *reinterpret_cast<const u32x4_a1*>(x + (xo[e] + k));
 #pragma unroll
-      for (int e = 0; e < WE; e++) wr[b][e] = *reinterpret_cast<const u32x4_a1*>(wp[e] + k);
+      for (int e = 0; e < WE; e++) wr[b][e] = *reinterpret_cast<const u32x4_a1*>(w + (wo[e] + k));
     } else {
 #pragma unroll
-      for (int e = 0; e < XE; e++) xr[b][e] = i8_load16(xp[e], k, K);
+      for (int e = 0; e < XE; e++) xr[b][e] = i8_load16(x + xo[e], (int)k, K);
 #pragma unroll
-      for (int e = 0; e < WE; e++) wr[b][e] = i8_load16(wp[e], k, K);
+      for (int e = 0; e < WE; e++) wr[b][e] = i8_load16(w + wo[e], (int)k, K);
     }
   };
   auto put = [&](int b, int o) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < XE; e++) *reinterpret_cast<u32x4*>(buf + o + slot + e * 4096) = xr[b][e];
+    for (int e = 0; e < XE; e++) *reinterpret_cast<u32x4*>(smem + o + slot + e * (RL * 128)) = xr[b][e];
 #pragma unroll
-    for (int e = 0; e < WE; e++) *reinterpret_cast<u32x4*>(buf + o + BM * 128 + slot + e * 4096) = wr[b][e];
+    for (int e = 0; e < WE; e++) *reinterpret_cast<u32x4*>(smem + o + BM * 128 + slot + e * (RL * 128)) = wr[b][e];
   };
   const int c0 = r16 * 128 + (q4 ^ (r16 & 7)) * 16;
   i32x4 acc[R][4];
@@ -664,44 +667,50 @@ __global__ __launch_bounds__(256, 2) void gemm_i8_any_kernel(const GemmI8Args a,
   for (int i = 0; i < R; i++)
 #pragma unroll
     for (int j = 0; j < 4; j++) acc[i][j] = zero_acc_i8();
-  // K step ks is in buffer b; register set b (steps of the same parity) holds step ks + 2 on its way, the other one step ks + 1
+  // K step ks is in buffer b; the registers hold step ks + 1 (D = 2: set 1 - b) and, on its way, step ks + 2
   auto step = [&](auto B, int ks) __attribute__((always_inline)) {
-    constexpr int b = decltype(B)::value, o = b * STG;
+    constexpr int b = decltype(B)::value, o = b * STG, set = D == 2 ? 1 - b : 0;
     if (ks < ks1) {
 #pragma unroll
       for (int kc = 0; kc < 2; kc++) {
-        u32x4 xa[R], wa[4];
+        u32x4 wa[4];
 #pragma unroll
-        for (int i = 0; i < R; i++) xa[i] = *reinterpret_cast<const u32x4*>(buf + o + (c0 ^ (kc * 64)) + (rw * R + i) * 2048);
+        for (int j = 0; j < 4; j++) wa[j] = *reinterpret_cast<const u32x4*>(smem + o + BM * 128 + (c0 ^ (kc * 64)) + (cw * 4 + j) * 2048);
 #pragma unroll
-        for (int j = 0; j < 4; j++) wa[j] = *reinterpret_cast<const u32x4*>(buf + o + BM * 128 + (c0 ^ (kc * 64)) + (cw * 4 + j) * 2048);
+        for (int i0 = 0; i0 < R; i0 += 4) {
+          u32x4 xa[R < 4 ? R : 4];
 #pragma unroll
-        for (int i = 0; i < R; i++)
+          for (int i = 0; i < (R < 4 ? R : 4); i++) xa[i] = *reinterpret_cast<const u32x4*>(smem + o + (c0 ^ (kc * 64)) + (rw * R + i0 + i) * 2048);
 #pragma unroll
-          for (int j = 0; j < 4; j++) mfma_i8(acc[i][j], wa[j], xa[i]);
+          for (int i = 0; i < (R < 4 ? R : 4); i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) mfma_i8(acc[i0 + i][j], wa[j], xa[i]);
+        }
       }
     }
-    if (ks + 1 < ks1) put(1 - b, STG - o);
-    load(1 - b, ks + 3);
+    if (ks + 1 < ks1) put(set, STG - o);
+    load(set, ks + 1 + D);
     __syncthreads();
   };
   load(0, ks0);
-  load(1, ks0 + 1);
+  if (D == 2) load(D - 1, ks0 + 1);
   put(0, 0);
-  load(0, ks0 + 2);
+  load(0, ks0 + D);
   __syncthreads();
   for (int ks = ks0; ks < ks1; ks += 2) {
     step(std::integral_constant<int, 0>{}, ks);
     step(std::integral_constant<int, 1>{}, ks + 1);
   }
   VRA_MFMA_DRAIN();
-  if (g.slices > 1) {
-    int v[R * 16];
+  if constexpr (R <= 4) {
+    if (g.slices > 1) {
+      int v[R * 16];
 #pragma unroll
-    for (int i = 0; i < R * 16; i++) v[i] = acc[i >> 4][i >> 2 & 3][i & 3];
-    if (!i8_meet<R * 16, 256>(v, g.ws, lin, tiles, z, g.slices)) return;
+      for (int i = 0; i < R * 16; i++) v[i] = acc[i >> 4][i >> 2 & 3][i & 3];
+      if (!i8_meet<R * 16, NT>(v, g.ws, lin, tiles, z, g.slices)) return;
 #pragma unroll
-    for (int i = 0; i < R * 16; i++) acc[i >> 4][i >> 2 & 3][i & 3] = v[i];
+      for (int i = 0; i < R * 16; i++) acc[i >> 4][i >> 2 & 3][i & 3] = v[i];
+    }
   }
   i8_store_rows<PAIR, R>(a, m0 + rw * R * 16 + r16, n0 + (PAIR ? cw * 32 : cw * 64), q4, acc);
 #endif

@@ -22,7 +22,7 @@ bool few_has(bool pair, int M, int C) {
   return pair ? (C == 2 && MT <= 4) || (C == 4 && MT <= 2) || (C == 8 && MT == 1) : (C == 1 || C == 2 ? MT <= 4 : C == 4 && MT <= 2);
 }
 int64_t tile_count(int M, int N, bool pair, int t) { return over(M, (t >> 4) * 64) * over(N, (t & 15) * (pair ? 32 : 64)); }
-bool any_has(int t) { return t == 0x11 || t == 0x22; }
+bool any_has(int t) { return t == 0x11 || t == 0x22 || t == 0x44; }
 int64_t tile_bytes(int t) { return (t >> 4) * (t & 15) * 16384; }  // of its sums
 bool tile_has(int t) { return t == 0x12 || t == 0x22 || t == 0x32 || t == 0x24 || t == 0x34 || t == 0x44; }
 // whether `slices` runs of K have a step each and meet within the workspace
@@ -61,20 +61,21 @@ double tile_us(bool pair, int M, int N, int K, int t, int slices) {
   const double us = std::max(c->t0 + (full + (rem > 0)) * c->round + steps * fill * (full * c->full + last), 3.0 + (pair ? 2.0 : 1.0) * N * K / 6.3e6);
   return slices == 1 ? us : us + c->meet + c->slice * slices + c->mb * wgs * rows * bn * 8e-6;
 }
-// rows that begin anywhere, 850 times of 1..8192 rows, rms 13..15 %, the choice 2.4 % behind the best on average: the same forms.  any: two workgroups a CU, a K step's time a constant
-// and one for each of the CU's workgroups
+// rows that begin anywhere, 859 times of 1..8192 rows, rms 6..16 %, the choice 2.6 % behind the best on average: the same forms.  any: 64 x 64 and 128 x 128 two workgroups a CU, a K step's time a
+// constant and one for each of the CU's workgroups
 double few_any_us(bool pair, int M, int N, int K) {
   const double t = pair ? 2 : 1, wgs = (double)over(N, 16);
-  return 3.3 + t * N * K / 11.1e6 + wgs * M * K / 8.6e6 + (double)over((int64_t)wgs, 256) * (16.0 * t + M) * K / 14.6e3;
+  return 3.1 + t * N * K / 10.6e6 + wgs * M * K / 8.3e6 + (double)over((int64_t)wgs, 256) * (16.0 * t + M) * K / 14.9e3;
 }
 double any_us(bool pair, int M, int N, int K, int t, int slices) {
+  struct Times { int slots; double t0, round, one, each, meet, slice; };
+  static const Times times[3] = {{512, 0.4, 3.7, 0.40, 0.27, 1.0, 0.99}, {512, 7.5, 0.0, 0.0, 1.107, 0.8, 1.84}, {256, 1.5, 9.9, 2.26, 0.05, 0.0, 0.0}};
+  const Times& c = times[t == 0x11 ? 0 : t == 0x22 ? 1 : 2];
   const int64_t wgs = tile_count(M, N, pair, t) * slices;
-  const bool small = t == 0x11;
-  const double steps = (double)over(K, 128) / slices, one = small ? 0.40 : 0.0, each = small ? 0.264 : 1.107, round = small ? 3.0 : 0.0;
-  const double full = (double)(wgs / 512), rem = (double)(wgs % 512);
-  double us = (small ? 1.1 : 7.4) + full * (round + steps * (one + 2.0 * each));
-  if (rem > 0) us += round + steps * (one + each * std::max(1.0, rem / 256));
-  if (slices > 1) us += small ? 0.6 + 1.0 * slices : 1.0 + 1.76 * slices;
+  const double steps = (double)over(K, 128) / slices, full = (double)(wgs / c.slots), rem = (double)(wgs % c.slots);
+  double us = c.t0 + full * (c.round + steps * (c.one + c.each * c.slots / 256));
+  if (rem > 0) us += c.round + steps * (c.one + c.each * std::max(1.0, rem / 256));
+  if (slices > 1) us += c.meet + c.slice * slices;
   return std::max(us, 3.0 + (pair ? 2.0 : 1.0) * N * K / 5.0e6);
 }
 
@@ -87,8 +88,8 @@ Choice choose(bool pair, int M, int N, int K, bool workspace, bool sixteens) {
   if (!sixteens && M <= 64) offer(I8_FEW, pair ? 2 : 1, 1, few_any_us(pair, M, N, K));
   for (int slices = 1; slices <= (workspace ? 8 : 1); slices *= 2) {
     if (!sixteens) {
-      for (const int t : {0x11, 0x22})
-        if (slices_fit(slices, K, tile_count(M, N, pair, t), tile_bytes(t))) offer(I8_ANY, t, slices, any_us(pair, M, N, K, t, slices));
+      for (const int t : {0x11, 0x22, 0x44})
+        if (t <= 0x22 ? slices_fit(slices, K, tile_count(M, N, pair, t), tile_bytes(t)) : slices == 1) offer(I8_ANY, t, slices, any_us(pair, M, N, K, t, slices));
       continue;
     }
     if (M <= 64)
@@ -116,20 +117,33 @@ void few_rows(const GemmI8Args& a, void* ws, int slices, hipStream_t st) {
   if constexpr (most >= 4) a.M <= 48 ? few<PAIR, 3, C, ANY>(a, ws, slices, st) : few<PAIR, 4, C, ANY>(a, ws, slices, st);
 }
 
-template <bool PAIR, int BM, int BN, bool DEEP>
-void tile(const GemmI8Args& a, void* ws, int slices, hipStream_t st) {
-  using G = GrTile<BM, BN, DEEP>;
-  constexpr int BC = PAIR ? BN / 2 : BN;
-  const GemmI8Tiles g = {ws, (a.M + BM - 1) / BM, (a.N + BC - 1) / BC, slices};
-  void (*const k)(GemmI8Args, GemmI8Tiles) = gemm_i8_tile_kernel<PAIR, BM, BN, DEEP>;
+// launches on up to 160 KB of LDS
+template <auto KERNEL>
+void launch_lds(unsigned grid, int threads, size_t lds, const GemmI8Args& a, const GemmI8Tiles& g, hipStream_t st) {
   static uint64_t attr_devs = 0;  // function attributes belong to the device current at the call
   int dev = 0;
   (void)hipGetDevice(&dev);
   if (!((__atomic_load_n(&attr_devs, __ATOMIC_RELAXED) >> (dev & 63)) & 1)) {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     __atomic_fetch_or(&attr_devs, (uint64_t)1 << (dev & 63), __ATOMIC_RELAXED);
   }
-  k<<<(unsigned)(g.MT * g.NT * slices), 512, (size_t)G::S * G::KP * G::STG, st>>>(a, g);
+  KERNEL<<<grid, threads, lds, st>>>(a, g);
+}
+template <bool PAIR, int BM, int BN>
+GemmI8Tiles tiles_of(const GemmI8Args& a, void* ws, int slices) {
+  constexpr int BC = PAIR ? BN / 2 : BN;
+  return {ws, (a.M + BM - 1) / BM, (a.N + BC - 1) / BC, slices};
+}
+template <bool PAIR, int BM, int BN, bool DEEP>
+void tile(const GemmI8Args& a, void* ws, int slices, hipStream_t st) {
+  using G = GrTile<BM, BN, DEEP>;
+  const GemmI8Tiles g = tiles_of<PAIR, BM, BN>(a, ws, slices);
+  launch_lds<gemm_i8_tile_kernel<PAIR, BM, BN, DEEP>>((unsigned)(g.MT * g.NT * slices), 512, (size_t)G::S * G::KP * G::STG, a, g, st);
+}
+template <bool PAIR, int BM, int BN, int NT, int D>
+void any(const GemmI8Args& a, void* ws, int slices, hipStream_t st) {
+  const GemmI8Tiles g = tiles_of<PAIR, BM, BN>(a, ws, slices);
+  launch_lds<gemm_i8_any_kernel<PAIR, BM, BN, NT, D>>((unsigned)(g.MT * g.NT * slices), NT, (size_t)2 * (BM + BN) * 128, a, g, st);
 }
 
 template <bool PAIR>
@@ -152,10 +166,9 @@ void run(const GemmI8Args& a, void* ws, const Choice& c, hipStream_t st) {
     if (tile_count(a.M, a.N, PAIR, 0x12) * c.slices <= 256) return tile<PAIR, 64, 128, true>(a, ws, c.slices, st);
     return tile<PAIR, 64, 128, false>(a, ws, c.slices, st);
   }
-  const GemmI8Tiles g = {ws, (int)over(a.M, (c.size >> 4) * 64), (int)over(a.N, (c.size & 15) * (PAIR ? 32 : 64)), c.slices};
-  const unsigned grid = (unsigned)(g.MT * g.NT * c.slices);
-  if (c.size == 0x22) gemm_i8_any_kernel<PAIR, 128, 128><<<grid, 256, 0, st>>>(a, g);
-  else gemm_i8_any_kernel<PAIR, 64, 64><<<grid, 256, 0, st>>>(a, g);
+  if (c.size == 0x44) return any<PAIR, 256, 256, 512, 1>(a, ws, c.slices, st);
+  if (c.size == 0x22) return any<PAIR, 128, 128, 256, 2>(a, ws, c.slices, st);
+  any<PAIR, 64, 64, 256, 2>(a, ws, c.slices, st);
 }
 
 void launch(GemmI8Args a, bool pair, void* ws, hipStream_t st) {
@@ -232,7 +245,7 @@ extern "C" void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x
   } else if (c.kind == I8_TILE) {
     has = has && tile_has(c.size) && in_sixteens(a) && (c.size <= 0x32 ? slices_fit(c.slices, k, tile_count(m, n, pair, c.size), tile_bytes(c.size)) : c.slices == 1);
   } else {
-    has = has && c.kind == I8_ANY && any_has(c.size) && slices_fit(c.slices, k, tile_count(m, n, pair, c.size), tile_bytes(c.size));
+    has = has && c.kind == I8_ANY && any_has(c.size) && (c.size <= 0x22 ? slices_fit(c.slices, k, tile_count(m, n, pair, c.size), tile_bytes(c.size)) : c.slices == 1);
   }
   VRA_CHECK_ARG(has, "vra_w8a8_gemm_on: no such kernel for this product");
   if (pair) run<true>(a, workspace, c, as_stream(stream));
