@@ -181,6 +181,22 @@ def test_rows_that_are_not_finite(cols):
     assert np.isnan(sc[2]) and not q[2].any()
 
 
+def part_of(buf, at, n, dtype):
+    """n elements of a device buffer from element `at` on"""
+    out = np.empty(n, dtype)
+    ops.lib().vra_device_sync()
+    ops.lib().vra_memcpy_d2h(out.ctypes.data, buf.ptr + at * out.itemsize, out.nbytes, 0)
+    ops.lib().vra_device_sync()
+    return out
+
+
+def test_more_rows_than_a_launch_takes():
+    r, T, H = rng(3), (1 << 20) + 37, 3
+    x, res, w = plain.to(r.standard_normal((T, H)), BF16), plain.to(r.standard_normal((T, H)), BF16), plain.to(1 + 0.2 * r.standard_normal(H), BF16)
+    for kind in ("quant", "add"):
+        check_rows(kind, x, BF16, rows_of(kind, x, BF16, res, w), res, w)
+
+
 # ---------------------------------------------------------------- products
 def some_codes(r, rows, cols):
     q = np.clip(np.rint(r.standard_normal((rows, cols)) * 40), -128, 127).astype(np.int8)
@@ -346,6 +362,24 @@ def test_scales_that_are_zero_or_nan(M, work):
     xs[0], xs[1] = 0.0, np.nan
     got = plain.wide(product(r, M, K, N, BF16, tensors=[x, xs, w, ws], work=work)[0], BF16)
     assert (got[0] == 0).all() and np.isnan(got[1]).all() and np.isfinite(got[2:]).all()
+
+
+def test_more_tiles_than_a_launch_takes():
+    """2^28 rows of one element: the launch is cut behind 2^22 tiles of 64 rows; the last rows of the first part and the second part"""
+    L, M, cut = ops.lib(), (1 << 28) + 70, 1 << 28
+    x, xs, res, out = ops.DevBuf(M), ops.DevBuf(M * 4), ops.DevBuf(M * 2), Guarded(M * 2)
+    L.vra_fill_hash_u32(x.ptr, M // 4, 3, 0)
+    L.vra_memset(x.ptr + M // 4 * 4, 5, M % 4, 0)
+    L.vra_fill_normal(xs.ptr, M, 4, 0.0, 1.0, F32, 0)
+    L.vra_fill_normal(res.ptr, M, 5, 0.0, 1.0, BF16, 0)
+    w, ws = np.full((1, 1), -77, np.int8), np.full(1, 0.01, np.float32)
+    wd, sd = ops.dev(w), ops.dev(ws)
+    L.vra_w8a8_gemm(x.ptr, xs.ptr, wd.ptr, sd.ptr, None, res.ptr, out.at, None, M, 1, 1, BF16, 0)
+    ops.check_error()
+    for at, n in ((0, 500), (cut - 300, 370)):
+        ref, bound = plain.gemm(part_of(x, at, n, np.int8)[:, None], part_of(xs, at, n, np.float32), w, ws, None, part_of(res, at, n, np.uint16)[:, None], BF16)
+        plain.assert_within(plain.wide(part_of(out, at, n, np.uint16)[:, None], BF16), ref, bound, f"rows from {at}")
+    assert (part_of(out, 2 * M, GUARD, np.uint8) == 0xA5).all()
 
 
 def test_wrappers():

@@ -52,6 +52,7 @@ __device__ __forceinline__ float i8_value(int g, int u, float xs, float gs, floa
   asm("" : "+v"(v));  // (the last product is not drawn into a conversion to f16, here or there: the bits are the same in all kernels)
   return v;
 }
+
 // rows begin anywhere: 16 bytes at a multiple of an element
 typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
 typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
@@ -203,15 +204,14 @@ __device__ __forceinline__ u32x4 i8_load16(const int8_t* row, int k, int K) {
 // 0.8 .. 1.7 us each, and a workgroup's waves waited for its last (150 x 3584, K = 18944, four slices of 128 x 128: 31.4 us, so 26.8; 32 x 512, K = 14336, eight slices: 8.9, 7.6).
 template <int V, int THREADS>
 __device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int tiles, int z, int slices) {
-  constexpr int W = V % 4 ? 1 : 4, B = V <= 16 ? 4 : V <= 32 ? 3 : 2;  // sums a load; slices in flight
+  static_assert(V % 4 == 0, "16 bytes a lane");
+  constexpr int B = V <= 16 ? 4 : V <= 32 ? 3 : 2;  // slices in flight
   const int tid = threadIdx.x;
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(static_cast<char*>(ws) + I8_WS_PARTIALS, 0, 0x7FFFFFF0, 0x00020000u);
-  auto at = [&](int s, int i) { return (uint32_t)(((s * tiles + tile) * (V / W) + i) * THREADS + tid) * (4u * W); };
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(static_cast<char*>(ws) + I8_WS_PARTIALS, 0, (int)I8_WS_PARTIAL_BYTES, 0x00020000u);
+  auto at = [&](int s, int i) { return (uint32_t)(((s * tiles + tile) * (V / 4) + i) * THREADS + tid) * 16u; };
 #pragma unroll
-  for (int i = 0; i < V / W; i++) {
-    if constexpr (W == 4) __builtin_amdgcn_raw_buffer_store_b128(u32x4{(uint32_t)v[4 * i], (uint32_t)v[4 * i + 1], (uint32_t)v[4 * i + 2], (uint32_t)v[4 * i + 3]}, r, at(z, i), 0, 16);
-    else __builtin_amdgcn_raw_buffer_store_b32((uint32_t)v[i], r, at(z, i), 0, 16);
-  }
+  for (int i = 0; i < V / 4; i++)
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4{(uint32_t)v[4 * i], (uint32_t)v[4 * i + 1], (uint32_t)v[4 * i + 2], (uint32_t)v[4 * i + 3]}, r, at(z, i), 0, 16);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   uint32_t* const count = static_cast<uint32_t*>(ws) + (tile * 8 + (tid >> 6)) * 16;
   uint32_t before = 0u;
@@ -220,15 +220,12 @@ __device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int til
   asm volatile("" ::: "memory");
   if (before != (uint32_t)slices - 1u) return false;
   for (int s0 = 1; s0 < slices; s0 += B) {
-    u32x4 p[B][(V + 3) / 4];
+    u32x4 p[B][V / 4];
 #pragma unroll
     for (int b = 0; b < B; b++) {
       const int s = z + s0 + b, o = s0 + b < slices ? (s >= slices ? s - slices : s) : z;  // (behind the last: its own again, not added)
 #pragma unroll
-      for (int i = 0; i < V / W; i++) {
-        if constexpr (W == 4) p[b][i] = __builtin_amdgcn_raw_buffer_load_b128(r, at(o, i), 0, 16);
-        else p[b][i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b32(r, at(o, i), 0, 16);
-      }
+      for (int i = 0; i < V / 4; i++) p[b][i] = __builtin_amdgcn_raw_buffer_load_b128(r, at(o, i), 0, 16);
     }
 #pragma unroll
     for (int b = 0; b < B; b++)
