@@ -276,7 +276,7 @@ def test_named_kernels(kind, size, slices, pair, work):
     rows = [1, 15, 16, 17, 33, 48, 64] if kind == 1 else [1, blocks - 1, blocks, blocks + 1, 2 * blocks + 3]
     for i, M in enumerate(rows):
         for j, (K, N) in enumerate([(1024, 300), (1168, 257), (1408, 64), (2032, 516), (3216, 8)] if kind == 1 or slices > 1 else [(128, 300), (16, 257), (384, 64), (496, 516), (656, 8)]):
-            K += 3 * (kind == 0 and j < 4)
+            K += 3 * (j < 4 and kind == 0 or j % 2 and (kind, size) == (1, 2 if pair else 1))
             dt = [BF16, F16, BF16 if pair else F32][(i + j) % 3]
             x, xs = some_codes(r, M, K)
             w, ws = some_codes(r, N, K)

@@ -61,21 +61,22 @@ double tile_us(bool pair, int M, int N, int K, int t, int slices) {
   const double us = std::max(c->t0 + (full + (rem > 0)) * c->round + steps * fill * (full * c->full + last), 3.0 + (pair ? 2.0 : 1.0) * N * K / 6.3e6);
   return slices == 1 ? us : us + c->meet + c->slice * slices + c->mb * wgs * rows * bn * 8e-6;
 }
-// rows that begin anywhere, 859 times of 1..8192 rows, rms 6..16 %, the choice 2.6 % behind the best on average: the same forms.  any: 64 x 64 and 128 x 128 two workgroups a CU, a K step's time a
+// rows that begin anywhere, 1020 times of 1..8192 rows, rms 6..14 %, the choice 2.2 % behind the best on average, 39 % at most (4 rows x 5632 + 5632, K = 2001): the same forms.  any: 64 x 64 and 128 x 128 two workgroups a CU, a K step's time a
 // constant and one for each of the CU's workgroups
-double few_any_us(bool pair, int M, int N, int K) {
+double few_any_us(bool pair, int M, int N, int K, int slices) {
   const double t = pair ? 2 : 1, wgs = (double)over(N, 16);
-  return 3.1 + t * N * K / 10.6e6 + wgs * M * K / 8.3e6 + (double)over((int64_t)wgs, 256) * (16.0 * t + M) * K / 14.9e3;
+  const double us = 3.2 + t * N * K / 8.9e6 + wgs * M * K / 9.4e6 + (double)over((int64_t)wgs * slices, 256) * (16.0 * t + M) * K / slices / 15.1e3;
+  return slices == 1 ? us : us + 1.54 + slices * (0.04 + 0.67 * over(M, 16) * 16 * N * t * 8e-6);
 }
 double any_us(bool pair, int M, int N, int K, int t, int slices) {
-  struct Times { int slots; double t0, round, one, each, meet, slice; };
-  static const Times times[3] = {{512, 0.4, 3.7, 0.40, 0.27, 1.0, 0.99}, {512, 7.5, 0.0, 0.0, 1.107, 0.8, 1.84}, {256, 1.5, 9.9, 2.26, 0.05, 0.0, 0.0}};
+  struct Times { int slots; double t0, round, one, each, meet, slice, mb; };
+  static const Times times[3] = {{512, 3.0, 0.9, 0.322, 0.372, 0.65, 0.78, 0.276}, {512, 7.5, 0.0, 0.026, 1.07, 0.0, 1.56, 0.202}, {256, 1.5, 9.9, 2.26, 0.05, 0, 0, 0}};
   const Times& c = times[t == 0x11 ? 0 : t == 0x22 ? 1 : 2];
   const int64_t wgs = tile_count(M, N, pair, t) * slices;
   const double steps = (double)over(K, 128) / slices, full = (double)(wgs / c.slots), rem = (double)(wgs % c.slots);
   double us = c.t0 + full * (c.round + steps * (c.one + c.each * c.slots / 256));
   if (rem > 0) us += c.round + steps * (c.one + c.each * std::max(1.0, rem / 256));
-  if (slices > 1) us += c.meet + c.slice * slices;
+  if (slices > 1) us += c.meet + c.slice * slices + c.mb * wgs * ((double)M / over(M, (t >> 4) * 64)) * (t & 15) * 64 * 8e-6;
   return std::max(us, 3.0 + (pair ? 2.0 : 1.0) * N * K / 5.0e6);
 }
 
@@ -85,9 +86,10 @@ Choice choose(bool pair, int M, int N, int K, bool workspace, bool sixteens) {
   auto offer = [&](int kind, int size, int slices, double v) {
     if (us == 0.0 || v < us) best = Choice{kind, size, slices}, us = v;
   };
-  if (!sixteens && M <= 64) offer(I8_FEW, pair ? 2 : 1, 1, few_any_us(pair, M, N, K));
   for (int slices = 1; slices <= (workspace ? 8 : 1); slices *= 2) {
     if (!sixteens) {
+      const int one = pair ? 2 : 1;
+      if (M <= 64 && slices_fit(slices, K, few_tiles(N, pair, one), few_bytes(pair, M, one))) offer(I8_FEW, one, slices, few_any_us(pair, M, N, K, slices));
       for (const int t : {0x11, 0x22, 0x44})
         if (t <= 0x22 ? slices_fit(slices, K, tile_count(M, N, pair, t), tile_bytes(t)) : slices == 1) offer(I8_ANY, t, slices, any_us(pair, M, N, K, t, slices));
       continue;
@@ -241,7 +243,7 @@ extern "C" void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x
   const Choice c = {kernel >> 8 & 255, kernel & 255, kernel >> 16};
   bool has = !(pair && (bias || residual)) && (int64_t)m * n <= (int64_t)1 << 34 && c.slices >= 1 && (c.slices == 1 || workspace);
   if (c.kind == I8_FEW) {
-    has = has && few_has(pair, m, c.size) && slices_fit(c.slices, k, few_tiles(n, pair, c.size), few_bytes(pair, m, c.size)) && (in_sixteens(a) || (c.size == (pair ? 2 : 1) && c.slices == 1));
+    has = has && few_has(pair, m, c.size) && slices_fit(c.slices, k, few_tiles(n, pair, c.size), few_bytes(pair, m, c.size)) && (in_sixteens(a) || c.size == (pair ? 2 : 1));
   } else if (c.kind == I8_TILE) {
     has = has && tile_has(c.size) && in_sixteens(a) && (c.size <= 0x32 ? slices_fit(c.slices, k, tile_count(m, n, pair, c.size), tile_bytes(c.size)) : c.slices == 1);
   } else {
