@@ -201,7 +201,7 @@ __device__ __forceinline__ u32x4 i8_load16(const int8_t* row, int k, int K) {
 // A wave stores its V sums a lane of slice z and counts itself; the last of the `slices` waves of the same place of the tile adds the others' sums to its own, sets the counter back and
 // returns true.  Nobody waits for anybody, and where slices end together their waves share the work.  Sums go through memory with agent scope (sc1: the L2s of the XCDs are
 // not coherent); a wave's stores are acknowledged before it counts itself, and the last one reads behind all counts.  It asks for several slices at a time: one after the other they were
-// 0.8 .. 1.7 us each, and a workgroup's waves waited for its last (150 x 3584, K = 18944, four slices of 128 x 128: 31.4 us, so 26.8; 32 x 512, K = 14336, eight slices: 8.9, 7.6).
+// 0.8 .. 1.7 us each, and a workgroup's waves waited for its last (with the epilogue's change, 150 x 3584, K = 18944, four slices of 128 x 128: 31.4 us, so 26.8; 32 x 512, K = 14336, eight slices: 8.9, 7.6).
 template <int V, int THREADS>
 __device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int tiles, int z, int slices) {
   static_assert(V % 4 == 0, "16 bytes a lane");
