@@ -121,7 +121,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_i8_kernel(const RowsI8
   const float amax = __uint_as_float(top);
   if (tid == 0) {
     const double s = (double)amax / 127.0;
-    a.scales[row] = finite ? (float)(NORM ? s / sqrt(sum / cols + (double)a.eps) : s) : __uint_as_float(0x7fc00000u);
+    // (nothing but zeros: 0, also where eps = 0 makes the norm 0 / 0)
+    a.scales[row] = !finite ? __uint_as_float(0x7fc00000u) : top == 0u ? 0.f : (float)(NORM ? s / sqrt(sum / cols + (double)a.eps) : s);
   }
   // the lower end of the range is moved up by a power of two: 127 / a does not overflow, no remainder is lost below the normal range
   const bool tiny = __builtin_amdgcn_readfirstlane(amax < 0x1p-60f);
