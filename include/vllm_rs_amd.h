@@ -173,9 +173,9 @@ void vra_dense_frag_gemm_segments(const void* x, const void* wd, const void* con
  * 16-bit activations only; no call of its own stands behind these).
  * Rows to 8 bits: q[t, c] = rint(127 p / a), a = max_c |p|, scales[t] = a / 127, with p = x (vra_quant_rows_i8), p = x weight (vra_rms_norm_i8) or
  * p = h weight, h = round(x + residual), written to h_out (vra_add_rms_norm_i8; h_out may be x or residual); behind a norm scales[t] is a / (127 sqrt(mean_c h^2 + eps)).
- * q is the correctly rounded quotient (ties to even) of the products p, which are formed in f32 (exact where they are normal numbers of it).  A row of zeros:
- * scale 0; a row in which x, the sum or a product is not finite in f32: codes 0, scale NaN, and so NaN in every product of it.  The mean is formed in f64.
- * x, residual, weight, h_out: bf16/f16, contiguous, 1..131072 columns, on any element. */
+ * q is the correctly rounded quotient (ties to even) of the products p, which are formed in f32 (exact where they are normal numbers of it).  A row of zeros (with
+ * eps = 0 too): scale 0; a row in which x, the sum or a product is not finite in f32: codes 0, scale NaN, and so NaN in every product of it.  The mean is formed in f64.
+ * x, residual, weight, h_out: bf16/f16, contiguous, 1..131072 columns, on any element; eps 0 or above. */
 void vra_quant_rows_i8(const void* x, int8_t* q, float* scales, int32_t rows, int32_t cols, int32_t dtype, int64_t stream);
 void vra_rms_norm_i8(const void* x, const void* weight, int8_t* q, float* scales, int32_t tokens, int32_t hidden, float eps, int32_t dtype,
                      int64_t stream);

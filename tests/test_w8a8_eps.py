@@ -1,10 +1,10 @@
-"""The RMS norms with 8-bit output: rows of zeros whatever eps is."""
+"""The RMS norms with 8-bit output: rows of zeros whatever eps is, and the eps that they refuse."""
 import numpy as np
 import pytest
 
 from tests import w8a8_plain as plain
 from tests.util import BF16, F16, rng
-from vllm_rs_amd import ops
+from vllm_rs_amd import _lib, ops
 
 
 @pytest.mark.gpu
@@ -33,3 +33,17 @@ def check(h, w, eps, dt, q, s, zero):
     ref, want = plain.rms_norm(h[rest], w, eps, dt)
     assert np.array_equal(q[rest], ref)
     plain.assert_within(s[rest].astype(np.float64), want, plain.SCALE * np.abs(want) + 2.0 ** -149, "scales")
+
+
+@pytest.mark.parametrize("eps", [-1e-6, -1.0, float("nan"), float("-inf")])
+def test_refused(eps):
+    """(null pointers: without the refusal there is another one, and no launch)"""
+    L = _lib.load()
+    for fn, pointers in (("vra_rms_norm_i8", 4), ("vra_add_rms_norm_i8", 6)):
+        L.vra_clear_error()
+        getattr(L, fn)(*[None] * pointers, 1, 64, eps, BF16, 0)
+        assert "eps" in L.vra_last_error().decode()
+        L.vra_clear_error()
+        getattr(L, fn)(*[None] * pointers, 1, 64, 0.0, BF16, 0)
+        assert "null" in L.vra_last_error().decode()
+        L.vra_clear_error()

@@ -224,6 +224,7 @@ template <int MODE>
 void rows_i8(const char* who, const RowsI8Args& a, int dtype, int64_t stream) {
   VRA_CHECK_ARG(a.rows >= 0 && a.cols > 0 && a.cols <= 131072, "%s: rows >= 0 and 1..131072 columns (rows=%d columns=%d)", who, a.rows, a.cols);
   VRA_CHECK_ARG(dtype == VRA_BF16 || dtype == VRA_F16, "%s: dtype must be bf16/f16", who);
+  VRA_CHECK_ARG(a.eps >= 0.f, "%s: eps must be 0 or above (eps=%g)", who, (double)a.eps);  // (NaN is neither; with less a finite row could have the scale of one that is not)
   if (a.rows == 0) return;
   VRA_CHECK_ARG(a.x && a.q && a.scales && (MODE == QI_PLAIN || a.weight) && (MODE != QI_ADD_NORM || (a.residual && a.h_out)), "%s: null pointer", who);
   VRA_CHECK_ARG((((uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.weight | (uintptr_t)a.h_out) & 1) == 0 && ((uintptr_t)a.scales & 3) == 0,
