@@ -173,20 +173,25 @@ void run(const GemmI8Args& a, void* ws, const Choice& c, hipStream_t st) {
   any<PAIR, 64, 64, 256, 2>(a, ws, c.slices, st);
 }
 
-void launch(GemmI8Args a, bool pair, void* ws, hipStream_t st) {
-  // a launch stays within 2^32 threads: 2^22 tiles of 64 x 64
+// a launch stays within 2^32 threads, and the rows of its tiles within 2^31: 2^22 tiles of 64 x 64 (2^31 threads on the kernels that take most for a result: 64 x 32 of 256, 64 x 64 of 512);
+// what has slices has few tiles and is not cut.  kernel_of(part): the kernel of each part
+template <class F>
+void in_parts(GemmI8Args a, bool pair, void* ws, hipStream_t st, F kernel_of) {
   const int64_t most = std::max<int64_t>((((int64_t)1 << 22) / (a.N / 64 + 1) * 64) & ~(int64_t)255, 256);
-  const bool sixteens = in_sixteens(a);
   while (a.M > 0) {
     GemmI8Args part = a;
     part.M = (int)std::min<int64_t>(a.M, most);
-    const Choice c = choose(pair, part.M, a.N, a.K, ws != nullptr, sixteens);
+    const Choice c = kernel_of(part);
     if (pair) run<true>(part, ws, c, st);
     else run<false>(part, ws, c, st);
     const size_t by = (size_t)part.M * a.N * (a.dtype == VRA_F32 ? 4 : 2);
     a.x += (size_t)part.M * a.K, a.xs += part.M, a.out = static_cast<char*>(a.out) + by, a.M -= part.M;
     if (a.residual) a.residual = static_cast<const char*>(a.residual) + by;
   }
+}
+void launch(const GemmI8Args& a, bool pair, void* ws, hipStream_t st) {
+  const bool sixteens = in_sixteens(a);
+  in_parts(a, pair, ws, st, [&](const GemmI8Args& part) { return choose(pair, part.M, a.N, a.K, ws != nullptr, sixteens); });
 }
 
 bool product_ok(const char* who, const GemmI8Args& a, bool pair, const void* workspace) {
@@ -241,7 +246,7 @@ extern "C" void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x
   const GemmI8Args a = {x, x_scales, {w, w_up}, {w_scales, s_up}, bias, residual, out, m, n, k, dtype};
   if (!product_ok("vra_w8a8_gemm_on", a, pair, workspace) || m == 0) return;
   const Choice c = {kernel >> 8 & 255, kernel & 255, kernel >> 16};
-  bool has = !(pair && (bias || residual)) && (int64_t)m * n <= (int64_t)1 << 34 && c.slices >= 1 && (c.slices == 1 || workspace);
+  bool has = !(pair && (bias || residual)) && c.slices >= 1 && (c.slices == 1 || workspace);
   if (c.kind == I8_FEW) {
     has = has && few_has(pair, m, c.size) && slices_fit(c.slices, k, few_tiles(n, pair, c.size), few_bytes(pair, m, c.size)) && (in_sixteens(a) || c.size == (pair ? 2 : 1));
   } else if (c.kind == I8_TILE) {
@@ -250,6 +255,5 @@ extern "C" void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x
     has = has && c.kind == I8_ANY && any_has(c.size) && (c.size <= 0x22 ? slices_fit(c.slices, k, tile_count(m, n, pair, c.size), tile_bytes(c.size)) : c.slices == 1);
   }
   VRA_CHECK_ARG(has, "vra_w8a8_gemm_on: no such kernel for this product");
-  if (pair) run<true>(a, workspace, c, as_stream(stream));
-  else run<false>(a, workspace, c, as_stream(stream));
+  in_parts(a, pair, workspace, as_stream(stream), [&](const GemmI8Args&) { return c; });
 }
