@@ -174,8 +174,9 @@ void vra_dense_frag_gemm_segments(const void* x, const void* wd, const void* con
  * Rows to 8 bits: q[t, c] = rint(127 p / a), a = max_c |p|, scales[t] = a / 127, with p = x (vra_quant_rows_i8), p = x weight (vra_rms_norm_i8) or
  * p = h weight, h = round(x + residual), written to h_out (vra_add_rms_norm_i8; h_out may be x or residual); behind a norm scales[t] is a / (127 sqrt(mean_c h^2 + eps)).
  * q is the correctly rounded quotient (ties to even) of the products p, which are formed in f32 (exact where they are normal numbers of it).  A row of zeros (with
- * eps = 0 too): scale 0; a row in which x, the sum or a product is not finite in f32: codes 0, scale NaN, and so NaN in every product of it.  The mean is formed in f64.
- * x, residual, weight, h_out: bf16/f16, contiguous, 1..131072 columns, on any element; eps 0 or above. */
+ * eps = 0 too): scale 0; a row in which x, h or a product is not finite: codes 0, scale NaN, and so NaN in every product of it.  The mean is formed in f64.
+ * x, residual, weight, h_out: bf16/f16, contiguous, 1..131072 columns, on any element; eps 0 or above.  vra_quant_rows_i8 over the rows of a 16-bit weight [n, k] makes the w and
+ * w_scales that the products below take. */
 void vra_quant_rows_i8(const void* x, int8_t* q, float* scales, int32_t rows, int32_t cols, int32_t dtype, int64_t stream);
 void vra_rms_norm_i8(const void* x, const void* weight, int8_t* q, float* scales, int32_t tokens, int32_t hidden, float eps, int32_t dtype,
                      int64_t stream);
@@ -197,7 +198,8 @@ void vra_w8a8_gemm_on(int32_t kernel, const int8_t* x, const float* x_scales, co
                       const void* bias, const void* residual, void* out, void* workspace, int32_t m, int32_t k, int32_t n, int32_t dtype,
                       int64_t stream);
 /* `workspace` of both: this many bytes on a multiple of 16, zeroed ONCE by the caller, one per concurrent stream (a captured graph counts as the stream it is replayed
- * on); products of few rows split K over workgroups that meet in it.  Null: no such split; the results are the same bits either way. */
+ * on).  A product of any number of rows may split K over workgroups that meet in it (prompts of thousands of rows too), so products that can run at the same time never
+ * share one.  Null: no such split, which is slower where there are few tiles; the results are the same bits either way. */
 size_t vra_w8a8_workspace_bytes(void);
 
 /* candle_nn::RmsNorm::forward as used by NormX (src/models/layers/others.rs:11-29):

@@ -157,6 +157,33 @@ def test_largest_sums_on_tiles(kernel, work):
         assert (out.numpy(np.float32, (M, N)) == np.float32(-128.0 * v * K)).all()
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_a_block_from_16_bit_weights(dt):
+    """weights and their scales made by the rows' entry, and a feed-forward block on them: each step against its definition on the step's own inputs"""
+    r, T, H, F, eps = rng(21), 37, 512, 1376, float(np.float32(1e-5))
+    x, res, norm_w = (plain.to(t, dt) for t in (r.standard_normal((T, H)), r.standard_normal((T, H)), 1 + 0.2 * r.standard_normal(H)))
+    w16 = {"gate": plain.to(r.standard_normal((F, H)) / 20, dt), "up": plain.to(r.standard_normal((F, H)) / 20, dt), "down": plain.to(r.standard_normal((H, F)) / 30, dt)}
+    w16["down"][3] = 0  # a channel that is off
+    dev = {k: ops.quant_rows_i8(ops.dev(v), *v.shape, dt) for k, v in w16.items()}
+    host = {k: (dev[k][0].numpy(np.int8, v.shape), dev[k][1].numpy(np.float32, (len(v),))) for k, v in w16.items()}
+    for k, v in w16.items():
+        q, s = plain.quant_rows(v, dt)
+        assert np.array_equal(host[k][0], q)
+        plain.assert_within(host[k][1].astype(np.float64), s, plain.SCALE * s + 2.0 ** -149, k)
+    p = ops.W8A8()
+    h, q, s = ops.add_rms_norm_i8(ops.dev(x), ops.dev(res), ops.dev(norm_w), T, H, eps, dt)
+    act = p.gate_up_silu(q, s, *dev["gate"], *dev["up"], T, H, F, dtype=dt)
+    aq, a_s = ops.quant_rows_i8(act, T, F, dt)
+    out = p.gemm(aq, a_s, *dev["down"], T, F, H, residual=h, dtype=dt)
+    hb, qb, sb = h.numpy(np.uint16, (T, H)), q.numpy(np.int8, (T, H)), s.numpy(np.float32, (T,))
+    ab, aqb, asb = act.numpy(np.uint16, (T, F)), aq.numpy(np.int8, (T, F)), a_s.numpy(np.float32, (T,))
+    assert np.array_equal(qb, plain.rms_norm(hb, norm_w, eps, dt)[0]) and np.array_equal(aqb, plain.quant_rows(ab, dt)[0])
+    plain.assert_within(plain.wide(ab, dt), *plain.gate_up_silu(qb, sb, *host["gate"], *host["up"], dt), "pair")
+    got = out.numpy(np.uint16, (T, H))
+    plain.assert_within(plain.wide(got, dt), *plain.gemm(aqb, asb, *host["down"], None, hb, dt), "down")
+    assert np.array_equal(got[:, 3], hb[:, 3])
+
+
 # ---------------------------------------------------------------- past 4 GiB and 2^31 elements
 @pytest.mark.parametrize("M, K", [(1, 12288), (40, 12288), (300, 12288), (3, 12289)])
 def test_weights_past_4_gib(M, K, work):
