@@ -74,8 +74,8 @@ __device__ __forceinline__ void i8_four(const void* row, int n, int N, V& v) {
   }
 }
 // A wave's R blocks of 16 rows x 64 virtual columns: lane (r16, q4) holds columns 4 q4 .. + 3 of the four tiles of a block (acc[block][tile]), of its row r16.  m: that row in
-// block 0; n0: the wave's first column.  What is read of rows and columns is asked for together, the residual two blocks ahead (one after the other, they were 30
-// of a 256 x 256 tile's 39 us behind its loop); 16-bit results trade places between a row's four lanes and go out 16 bytes a lane.
+// block 0; n0: the wave's first column.  What is read of rows and columns is asked for together, the residual two blocks ahead;
+// 16-bit results trade places between a row's four lanes and go out 16 bytes a lane.
 template <class T, bool PAIR, int R>
 __device__ __forceinline__ void i8_store_rows(const GemmI8Args& a, int m, int n0, int q4, const i32x4 (&acc)[R][4]) {
   constexpr int NJ = PAIR ? 2 : 4;
@@ -201,7 +201,7 @@ __device__ __forceinline__ u32x4 i8_load16(const int8_t* row, int k, int K) {
 // A wave stores its V sums a lane of slice z and counts itself; the last of the `slices` waves of the same place of the tile adds the others' sums to its own, sets the counter back and
 // returns true.  Nobody waits for anybody, and where slices end together their waves share the work.  Sums go through memory with agent scope (sc1: the L2s of the XCDs are
 // not coherent); a wave's stores are acknowledged before it counts itself, and the last one reads behind all counts.  It asks for several slices at a time: one after the other they were
-// 0.8 .. 1.7 us each, and a workgroup's waves waited for its last (with the epilogue's change, 150 x 3584, K = 18944, four slices of 128 x 128: 31.4 us, so 26.8; 32 x 512, K = 14336, eight slices: 8.9, 7.6).
+// 0.8 .. 1.7 us each, and a workgroup's waves waited for its last (150 x 3584, K = 18944, four slices of 128 x 128: 29.4 us, so 28.0; 32 x 512, K = 14336, eight slices: 8.9, 7.6).
 template <int V, int THREADS>
 __device__ __forceinline__ bool i8_meet(int (&v)[V], void* ws, int tile, int tiles, int z, int slices) {
   static_assert(V % 4 == 0, "16 bytes a lane");
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(I8_NW * 64) void gemm_i8_few_kernel(const GemmI8Arg
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int M = a.M, N = a.N, K = a.K, tile = (int)blockIdx.x / slices, z = (int)blockIdx.x - tile * slices, n0 = tile * CO * 16;
   // a lane's two pieces of a step: one of each half, so that a request is for 64 bytes of a row.  It meets fewer lines than one for 128 where rows do not begin with one (pieces side by side / so:
-  // pair 11 x 9216, K = 9264 50.0 / 46.8 us, 11 x 17024, K = 4384 26.8 / 24.1; whole lines 1 % slower, and with the form by K 7 %, for its registers)
+  // pair 11 x 9216, K = 9264 49.9 / 47.4 us, 11 x 17024, K = 4384 26.9 / 24.2; whole lines 1 % slower, and with the form by K 7 %, for its registers)
   const int8_t* wp[C];
   const int8_t* xp[MT];
 #pragma unroll

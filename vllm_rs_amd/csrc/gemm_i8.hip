@@ -32,7 +32,7 @@ bool slices_fit(int slices, int K, int64_t tiles, int64_t tile_bytes) {
 int64_t few_bytes(bool pair, int M, int C) { return (int64_t)((M + 15) / 16) * C * 1024; }  // of a workgroup's sums
 
 // Times in us, fitted to 2018 (few) and 2957 (tile) measured ones: 1..64 and 17..8192 rows, 27 products of K = 992..18944 and 192..32000 columns, weights from memory; the
-// choice by them is 0.65 % behind the best one measured on average and 17 % at most (411 of 472 products, the others chose what was not measured).  Rows that are no whole lines of 128 bytes cost more on every way.
+// choice by them is 0.65 % behind the best one of the same times on average and 17 % at most (411 of 472 products, the others chose what was not measured; none was held out).  Rows that are no whole lines of 128 bytes cost more on every way.
 // few: what the busiest CU reads, at 36 GB/s, and the weights at 7.0 TB/s, the longer of them and a quarter of the other; the slices' meeting, for each of them and for each MB that they write and read
 double few_us(bool pair, int M, int N, int K, int C, int slices) {
   const double wgs = (double)few_tiles(N, pair, C) * slices, t = pair ? 2 : 1;
@@ -61,7 +61,7 @@ double tile_us(bool pair, int M, int N, int K, int t, int slices) {
   const double us = std::max(c->t0 + (full + (rem > 0)) * c->round + steps * fill * (full * c->full + last), 3.0 + (pair ? 2.0 : 1.0) * N * K / 6.3e6);
   return slices == 1 ? us : us + c->meet + c->slice * slices + c->mb * wgs * rows * bn * 8e-6;
 }
-// rows that begin anywhere, 1913 times of 176 products, 1..8192 rows, the choice 2.5 % behind the best on average, 39 % at most (4 rows x 5632 + 5632, K = 2001): the same forms.  any: 64 x 64 and 128 x 128 two workgroups a CU, a K step's time a
+// rows that begin anywhere, 1913 times of 176 products, 1..8192 rows, the choice 2.5 % behind the best of these on average, 39 % at most (4 rows x 5632 + 5632, K = 2001): the same forms.  any: 64 x 64 and 128 x 128 two workgroups a CU, a K step's time a
 // constant and one for each of the CU's workgroups
 double few_any_us(bool pair, int M, int N, int K, int slices) {
   const double t = pair ? 2 : 1, wgs = (double)over(N, 16);

@@ -5,7 +5,7 @@
 //
 // The norm's factor is the same for a whole row: it is in the scale, and not in q.  Products of two 16-bit floats are exact in f32, and a quotient within the
 // f32 division's error of a half is decided by its exact remainder: q is the definition's, bit for bit, whatever the order of the sums.
-// Bound: memory, and close behind it the vector instructions, 12 an element without a norm and 18 with one (8192 x 4096 bf16: sum and norm 44.5 us = 5.3 TB/s, norm 23.5 = 4.3;
+// Bound: memory, and close behind it the vector instructions, 12 an element without a norm and 18 with one (8192 x 4096 bf16: sum and norm 44.6 us = 5.3 TB/s, norm 23.5 = 4.3;
 // 3063 x 18944 f16 38.0 = 4.6).  A row is read once and kept in registers as it came (the sum as it is stored) between the reduction and the quotients.
 #include <type_traits>
 
